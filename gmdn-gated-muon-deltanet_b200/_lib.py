@@ -87,6 +87,27 @@ lib.gmdn_head_rmsnorm_fwd.argtypes = [_p] * 3 + [_i] * 4 + [ctypes.c_float] + [_
 lib.gmdn_head_rmsnorm_bwd.restype = _i
 lib.gmdn_head_rmsnorm_bwd.argtypes = [_p] * 5 + [_i] * 4 + [ctypes.c_float] + [_i] * 2 + [_p]
 
+_q = ctypes.c_longlong
+_f = ctypes.c_float
+lib.gmdn_norm_fwd.restype = _i
+lib.gmdn_norm_fwd.argtypes = [_p] * 8 + [_q, _i, _f] + [_i] * 4 + [_p]
+lib.gmdn_norm_bwd_workspace_bytes.restype = _z
+lib.gmdn_norm_bwd_workspace_bytes.argtypes = [_q, _i]
+lib.gmdn_norm_bwd.restype = _i
+lib.gmdn_norm_bwd.argtypes = [_p] * 11 + [_z, _q] + [_i] * 7 + [_p]
+lib.gmdn_token_logprobs_fwd.restype = _i
+lib.gmdn_token_logprobs_fwd.argtypes = [_p] * 7 + [_q] * 4 + [_i] * 2 + [_q, _i, _p]
+lib.gmdn_token_logprobs_bwd.restype = _i
+lib.gmdn_token_logprobs_bwd.argtypes = [_p] * 8 + [_q] * 4 + [_i] * 2 + [_q, _i, _p]
+lib.gmdn_pack8.restype = _i
+lib.gmdn_pack8.argtypes = [_p] * 3 + [_q, _i, _p]
+lib.gmdn_unpack8.restype = _i
+lib.gmdn_unpack8.argtypes = [_p] * 3 + [_q, _i, _p]
+lib.gmdn_act8_fwd.restype = _i
+lib.gmdn_act8_fwd.argtypes = [_p] * 7 + [_q, _i, _p]
+lib.gmdn_act8_bwd.restype = _i
+lib.gmdn_act8_bwd.argtypes = [_p] * 8 + [_q, _i, _p]
+
 
 def check(rc: int, what: str) -> None:
     """Raise RuntimeError carrying the library's message when rc != 0."""

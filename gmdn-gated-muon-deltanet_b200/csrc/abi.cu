@@ -16,6 +16,7 @@
 #include "../../include/gmdn_scan.h"
 #include "scan_kernels.h"
 #include "fast_path.h"
+#include "step_ops.h"
 
 namespace {
 
@@ -373,6 +374,210 @@ int gmdn_head_rmsnorm_bwd(const void* o, const float* weight, const void* dy, vo
   GMDN_LAUNCH(gmdn::head_rmsnorm_bwd(o, weight, dy, d_o, dweight, B, H, T, dh, e, in_f32 != 0,
                                      out_f32 != 0, st),
               "head_rmsnorm_bwd");
+  return GMDN_OK;
+}
+
+// ---- the training step around the mixer ---------------------------------------
+
+static bool misaligned(std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % 16) return true;
+  return false;
+}
+
+static int check_norm(const char* who, long long rows, int width) {
+  if (rows < 0 || width < 0)
+    return fail(GMDN_ERR_INVALID, "%s: negative size rows=%lld width=%d", who, rows, width);
+  if (width > 0 && rows > (1ll << 60) / width)
+    return fail(GMDN_ERR_UNSUPPORTED, "%s: too many elements", who);
+  return GMDN_OK;
+}
+
+int gmdn_norm_fwd(const void* x, const void* residual, const float* weight, const float* bias,
+                  void* y, void* h, float* rstd, float* mean, long long rows, int width, float eps,
+                  int center, int x_f32, int res_f32, int y_f32, void* stream) {
+  g_last_error.clear();
+  int rc = check_norm("norm", rows, width);
+  if (rc) return rc;
+  if (rows == 0 || width == 0) return GMDN_OK;
+  if (!x || !y || !rstd || (residual && !h) || (center && !mean))
+    return fail(GMDN_ERR_INVALID, "norm: null pointer");
+  if (misaligned({x, residual, weight, bias, y, h}))
+    return fail(GMDN_ERR_INVALID, "norm: pointers must be 16-byte aligned");
+  if (!(eps >= 0.f)) return fail(GMDN_ERR_INVALID, "norm: eps must be >= 0");
+  gmdn::NormFwdArgs p{x, residual, weight, bias, y, h, rstd, mean, rows, width, eps,
+                      center != 0, x_f32 != 0, res_f32 != 0, y_f32 != 0};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  GMDN_LAUNCH(gmdn::norm_fwd(p, st), "norm_fwd");
+  return GMDN_OK;
+}
+
+size_t gmdn_norm_bwd_workspace_bytes(long long rows, int width) {
+  if (rows <= 0 || width <= 0) return 0;
+  return static_cast<size_t>(gmdn::norm_bwd_partials(rows, width)) * 2 * width * sizeof(float);
+}
+
+int gmdn_norm_bwd(const void* s, const float* rstd, const float* mean, const float* weight,
+                  const void* dy, const void* dh, void* ds_a, void* ds_b, float* dweight,
+                  float* dbias, void* workspace, size_t workspace_bytes, long long rows, int width,
+                  int center, int s_f32, int dy_f32, int dh_f32, int a_f32, int b_f32,
+                  void* stream) {
+  g_last_error.clear();
+  int rc = check_norm("norm", rows, width);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0 || width == 0) {
+    for (float* d : {dweight, dbias})
+      if (d && width > 0) {
+        cudaError_t ce = cudaMemsetAsync(d, 0, sizeof(float) * width, st);
+        if (ce != cudaSuccess) return cuda_fail(ce, "norm_bwd");
+      }
+    return GMDN_OK;
+  }
+  if (!s || !rstd || !dy || (center && !mean)) return fail(GMDN_ERR_INVALID, "norm: null pointer");
+  if (misaligned({s, weight, dy, dh, ds_a, ds_b}))
+    return fail(GMDN_ERR_INVALID, "norm: pointers must be 16-byte aligned");
+  const size_t need = gmdn_norm_bwd_workspace_bytes(rows, width);
+  if ((dweight || dbias) && (!workspace || workspace_bytes < need))
+    return fail(GMDN_ERR_WORKSPACE, "workspace %zu bytes < required %zu", workspace_bytes, need);
+  gmdn::NormBwdArgs p{s, rstd, mean, weight, dy, dh, ds_a, ds_b, dweight, dbias,
+                      static_cast<float*>(workspace), rows, width, center != 0, s_f32 != 0,
+                      dy_f32 != 0, dh_f32 != 0, a_f32 != 0, b_f32 != 0};
+  GMDN_LAUNCH(gmdn::norm_bwd(p, st), "norm_bwd");
+  return GMDN_OK;
+}
+
+static int check_logprobs(const void* logits, long long batch, long long length, int vocab,
+                          int top_k, int f32) {
+  if (batch < 0 || length < 0 || vocab < 1)
+    return fail(GMDN_ERR_INVALID, "token_logprobs: bad size batch=%lld length=%lld vocab=%d", batch,
+                length, vocab);
+  if (length > 0 && batch > (1ll << 60) / length / vocab)
+    return fail(GMDN_ERR_UNSUPPORTED, "token_logprobs: too many elements");
+  if (top_k < 0 || top_k > gmdn::kMaxTopK || top_k > vocab)
+    return fail(GMDN_ERR_INVALID, "token_logprobs: top_k must be in [0, min(%d, vocab)] (got %d)",
+                gmdn::kMaxTopK, top_k);
+  if (batch * length > 0 && (!logits || reinterpret_cast<uintptr_t>(logits) % (f32 ? 4 : 2)))
+    return fail(GMDN_ERR_INVALID, "token_logprobs: null or misaligned logits");
+  return GMDN_OK;
+}
+
+int gmdn_token_logprobs_fwd(const void* logits, const int64_t* targets, float* logprobs,
+                            float* entropy, float* top_logprobs, int64_t* top_ids, float* stats,
+                            long long batch, long long length, long long stride_b,
+                            long long stride_t, int vocab, int top_k, int64_t ignore_index,
+                            int f32, void* stream) {
+  g_last_error.clear();
+  int rc = check_logprobs(logits, batch, length, vocab, top_k, f32);
+  if (rc) return rc;
+  if (batch * length == 0) return GMDN_OK;
+  if ((logprobs && !targets) || (top_k > 0 && (!top_logprobs || !top_ids)))
+    return fail(GMDN_ERR_INVALID, "token_logprobs: null pointer");
+  if (stats && reinterpret_cast<uintptr_t>(stats) % 16)
+    return fail(GMDN_ERR_INVALID, "token_logprobs: stats must be 16-byte aligned");
+  gmdn::LogprobArgs p{};
+  p.logits = logits; p.batch = batch; p.length = length;
+  p.stride_b = stride_b; p.stride_t = stride_t;
+  p.vocab = vocab; p.f32 = f32 != 0; p.targets = targets; p.ignore_index = ignore_index;
+  p.stats = stats; p.logprobs = logprobs; p.entropy = entropy; p.top_logprobs = top_logprobs;
+  p.top_ids = top_ids; p.top_k = top_k;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  GMDN_LAUNCH(gmdn::token_logprobs_fwd(p, st), "token_logprobs_fwd");
+  return GMDN_OK;
+}
+
+int gmdn_token_logprobs_bwd(const void* logits, const int64_t* targets, const float* stats,
+                            const int64_t* top_ids, const float* g_logprobs,
+                            const float* g_entropy, const float* g_top, void* dlogits,
+                            long long batch, long long length, long long stride_b,
+                            long long stride_t, int vocab, int top_k, int64_t ignore_index,
+                            int f32, void* stream) {
+  g_last_error.clear();
+  int rc = check_logprobs(logits, batch, length, vocab, top_k, f32);
+  if (rc) return rc;
+  if (batch * length == 0) return GMDN_OK;
+  if (!stats || !dlogits || (g_logprobs && !targets) || (g_top && !top_ids))
+    return fail(GMDN_ERR_INVALID, "token_logprobs: null pointer");
+  if (misaligned({stats, dlogits}))
+    return fail(GMDN_ERR_INVALID, "token_logprobs: stats and dlogits must be 16-byte aligned");
+  gmdn::LogprobArgs p{};
+  p.logits = logits; p.batch = batch; p.length = length;
+  p.stride_b = stride_b; p.stride_t = stride_t;
+  p.vocab = vocab; p.f32 = f32 != 0; p.targets = targets; p.ignore_index = ignore_index;
+  p.stats = const_cast<float*>(stats); p.top_ids = const_cast<int64_t*>(top_ids);
+  p.top_k = g_top ? top_k : 0;
+  p.g_logprobs = g_logprobs; p.g_entropy = g_entropy; p.g_top = g_top; p.dlogits = dlogits;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  GMDN_LAUNCH(gmdn::token_logprobs_bwd(p, st), "token_logprobs_bwd");
+  return GMDN_OK;
+}
+
+static int check_act8(const char* who, std::initializer_list<const void*> ptrs, long long n) {
+  if (n < 0 || n > (1ll << 60)) return fail(GMDN_ERR_INVALID, "%s: bad size %lld", who, n);
+  if (n == 0) return GMDN_OK;
+  for (const void* p : ptrs) {
+    if (!p) return fail(GMDN_ERR_INVALID, "%s: null pointer", who);
+    if (reinterpret_cast<uintptr_t>(p) % 16)
+      return fail(GMDN_ERR_INVALID, "%s: pointers must be 16-byte aligned", who);
+  }
+  return GMDN_OK;
+}
+
+int gmdn_pack8(const void* x, int8_t* codes, float* scales, long long n, int f32, void* stream) {
+  g_last_error.clear();
+  int rc = check_act8("pack8", {x, codes, scales}, n);
+  if (rc || n == 0) return rc;
+  gmdn::Act8Args p{};
+  p.x = x; p.codes = codes; p.scales = scales; p.n = n; p.f32 = f32 != 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  GMDN_LAUNCH(gmdn::pack8(p, st), "pack8");
+  return GMDN_OK;
+}
+
+int gmdn_unpack8(const int8_t* codes, const float* scales, void* x, long long n, int f32,
+                 void* stream) {
+  g_last_error.clear();
+  int rc = check_act8("unpack8", {codes, scales, x}, n);
+  if (rc || n == 0) return rc;
+  gmdn::Act8Args p{};
+  p.codes = const_cast<int8_t*>(codes); p.scales = const_cast<float*>(scales);
+  p.y = x; p.n = n; p.f32 = f32 != 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  GMDN_LAUNCH(gmdn::unpack8(p, st), "unpack8");
+  return GMDN_OK;
+}
+
+int gmdn_act8_fwd(const void* x, const void* gate, void* y, int8_t* codes, float* scales,
+                  int8_t* gate_codes, float* gate_scales, long long n, int f32, void* stream) {
+  g_last_error.clear();
+  int rc = check_act8("act8_fwd", {x, y, codes, scales}, n);
+  if (!rc && gate) rc = check_act8("act8_fwd", {gate, gate_codes, gate_scales}, n);
+  if (rc || n == 0) return rc;
+  gmdn::Act8Args p{};
+  p.x = x; p.gate = gate; p.y = y; p.codes = codes; p.scales = scales;
+  p.gate_codes = gate_codes; p.gate_scales = gate_scales; p.n = n; p.f32 = f32 != 0;
+  p.gated = gate != nullptr;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  GMDN_LAUNCH(gmdn::act8_fwd(p, st), "act8_fwd");
+  return GMDN_OK;
+}
+
+int gmdn_act8_bwd(const int8_t* codes, const float* scales, const int8_t* gate_codes,
+                  const float* gate_scales, const void* dy, void* dx, void* dgate, void* y,
+                  long long n, int f32, void* stream) {
+  g_last_error.clear();
+  int rc = check_act8("act8_bwd", {codes, scales, dy, dx}, n);
+  if (!rc && gate_codes) rc = check_act8("act8_bwd", {gate_scales, dgate}, n);
+  if (rc || n == 0) return rc;
+  if (misaligned({gate_codes, y}))
+    return fail(GMDN_ERR_INVALID, "act8_bwd: pointers must be 16-byte aligned");
+  gmdn::Act8Args p{};
+  p.codes = const_cast<int8_t*>(codes); p.scales = const_cast<float*>(scales);
+  p.gate_codes = const_cast<int8_t*>(gate_codes); p.gate_scales = const_cast<float*>(gate_scales);
+  p.dy = dy; p.dx = dx; p.dgate = dgate; p.y = y; p.n = n; p.f32 = f32 != 0;
+  p.gated = gate_codes != nullptr;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  GMDN_LAUNCH(gmdn::act8_bwd(p, st), "act8_bwd");
   return GMDN_OK;
 }
 

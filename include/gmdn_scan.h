@@ -226,6 +226,82 @@ int gmdn_head_rmsnorm_bwd(const void* o, const float* weight, const void* dy, vo
                           float* dweight, int B, int H, int T, int dh, float eps, int in_f32,
                           int out_f32, void* stream);
 
+/* ---- the training step around the mixer ------------------------------------
+ *
+ * Layer norm (center 1) or RMS norm (center 0) of s over the last axis of
+ * (rows, width), s = x or, with a residual, s = x + residual rounded to h's
+ * type (fp32 if x or residual is, else bf16) and written to h:
+ * y = (s - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps).  weight,
+ * bias (width, fp32) and residual / h may be NULL; rstd (and mean, with center)
+ * (rows, fp32) are kept for the backward.  *_f32: 1 = fp32, 0 = bf16.  Any width;
+ * tensor pointers 16-byte aligned.  What it replaces in the model: the
+ * nn.RMSNorm of each block and the residual add before it
+ * (train_ablation.py:197-246). */
+int gmdn_norm_fwd(const void* x, const void* residual, const float* weight, const float* bias,
+                  void* y, void* h, float* rstd, float* mean, long long rows, int width, float eps,
+                  int center, int x_f32, int res_f32, int y_f32, void* stream);
+
+/* Scratch bytes for gmdn_norm_bwd when it computes dweight or dbias. */
+size_t gmdn_norm_bwd_workspace_bytes(long long rows, int width);
+
+/* Backward: s is what was normalised (x, or h), dy the cotangent of y, dh that
+ * of h (NULL: none).  The gradient of s (dh included) is written to ds_a and
+ * ds_b in the type of each (either may be NULL: x and residual share it).
+ * dweight, dbias (width, fp32; either may be NULL) are overwritten; they are
+ * summed in a fixed order, so equal calls give equal bits. */
+int gmdn_norm_bwd(const void* s, const float* rstd, const float* mean, const float* weight,
+                  const void* dy, const void* dh, void* ds_a, void* ds_b, float* dweight,
+                  float* dbias, void* workspace, size_t workspace_bytes, long long rows, int width,
+                  int center, int s_f32, int dy_f32, int dh_f32, int a_f32, int b_f32,
+                  void* stream);
+
+/* Log probabilities of given tokens.  Row (b, t) of the logits, vocab
+ * contiguous elements (f32: 1 = fp32, 0 = bf16), starts at element
+ * b * stride_b + t * stride_t (any alignment).  For each row: logprobs =
+ * log softmax at targets (0 where the target is ignore_index, NaN where it is
+ * no column), entropy of the row, and the top_k (at most 64) largest logits'
+ * log probabilities and columns, in falling order, ties to the lowest column.
+ * Any output may be NULL; top_k 0 writes no alternatives.  stats (rows, 4 fp32)
+ * keeps what the backward needs, and may be NULL where there is none.  A row of
+ * nothing but -inf has logprob -inf, entropy 0 and a zero gradient; a row with
+ * a NaN or +inf gives NaN (its alternatives are columns 0, 1, ...).  The
+ * trainer's loss is its mean (train_ablation.py:197-246, 386-399). */
+int gmdn_token_logprobs_fwd(const void* logits, const int64_t* targets, float* logprobs,
+                            float* entropy, float* top_logprobs, int64_t* top_ids, float* stats,
+                            long long batch, long long length, long long stride_b,
+                            long long stride_t, int vocab, int top_k, int64_t ignore_index,
+                            int f32, void* stream);
+
+/* Backward: dlogits (batch, length, vocab) contiguous, in the logits' type,
+ * from the cotangents of logprobs, entropy (rows) and top_logprobs (rows,
+ * top_k), each of which may be NULL. */
+int gmdn_token_logprobs_bwd(const void* logits, const int64_t* targets, const float* stats,
+                            const int64_t* top_ids, const float* g_logprobs,
+                            const float* g_entropy, const float* g_top, void* dlogits,
+                            long long batch, long long length, long long stride_b,
+                            long long stride_t, int vocab, int top_k, int64_t ignore_index,
+                            int f32, void* stream);
+
+/* Activations in 8 bits.  Each 128 consecutive elements share a scale: with
+ * a = max|x|, codes = round_even(x * fp32(127 / a)) and an element comes back as
+ * code * fp32(a * fp32(1 / 127)): off by at most half a step a / 254 and
+ * rounding.  Blocks with a < 2^-100 come back as zeros, blocks with a NaN or an
+ * infinity as NaN.  codes n bytes, scales ceil(n / 128) fp32; all pointers
+ * 16-byte aligned.  No counterpart in the reference. */
+int gmdn_pack8(const void* x, int8_t* codes, float* scales, long long n, int f32, void* stream);
+int gmdn_unpack8(const int8_t* codes, const float* scales, void* x, long long n, int f32,
+                 void* stream);
+
+/* y = GELU(x) (gate NULL; exact, by the normal distribution) or SiLU(gate) * x,
+ * and the 8-bit checkpoint of x (and gate); the backward reads the checkpoint in
+ * place of x (and gate), writes dx (and dgate) and, unless y is NULL, the
+ * activation of the restored inputs (train_ablation.py:202-205, the MLP). */
+int gmdn_act8_fwd(const void* x, const void* gate, void* y, int8_t* codes, float* scales,
+                  int8_t* gate_codes, float* gate_scales, long long n, int f32, void* stream);
+int gmdn_act8_bwd(const int8_t* codes, const float* scales, const int8_t* gate_codes,
+                  const float* gate_scales, const void* dy, void* dx, void* dgate, void* y,
+                  long long n, int f32, void* stream);
+
 /* Failure-detection self-test (diagnostic; no reference counterpart): launches
  * one CTA whose bounded mbarrier wait -- the same wait the kernels use -- can
  * never complete, with a limit of limit_ns (clamped to [1 ms, 2 s]).  The wait
