@@ -32,7 +32,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from ._lib import check, lib
-from .ops import _aligned, _f32_flag, _ptr, _require_cuda, _stream
+from .ops import _aligned, _f32_flag, _require_cuda
 
 __all__ = ["layer_norm", "rms_norm", "token_logprobs", "TokenLogprobs", "pack8", "unpack8",
            "Packed8", "act8_forward", "act8_backward", "Act8Saved", "mlp8"]
@@ -48,11 +48,39 @@ def _eager(*tensors: Optional[Tensor]) -> bool:
             and all(t is None or type(t) in _PLAIN for t in tensors))
 
 
+def _run(what: str, fn, device: torch.device, *args) -> None:
+    """The library call on the device's current stream, with that device current."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, what)
+
+
+def _at(t: Optional[Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
 def _same_device(name: str, first: Tensor, *others: Optional[Tensor]) -> None:
     _require_cuda(name, first, *others)
     for t in others:
         if t is not None and t.device != first.device:
             raise ValueError(f"{name}: tensors on {first.device} and {t.device}")
+
+
+def _once(backward):
+    """A Function's backward without a second derivative: asking for one (grad
+    mode on) raises when it is used.  The wrapper that does this is left out
+    where grad mode is off, as in every plain backward."""
+    strict = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return strict(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return staticmethod(run)
 
 
 def _needs_grad(*tensors: Optional[Tensor]) -> bool:
@@ -68,19 +96,17 @@ def _norm_fwd_call(x: Tensor, residual: Optional[Tensor], weight: Optional[Tenso
                    out_f32: bool) -> tuple[Tensor, Tensor, Tensor]:
     D = x.shape[-1]
     rows = x.numel() // D if D else 0
-    y = torch.empty(x.shape, dtype=torch.float32 if out_f32 else torch.bfloat16, device=x.device)
+    y = torch.empty_like(x, dtype=torch.float32 if out_f32 else torch.bfloat16)
     if residual is None:
         h = x.new_empty(0)
     else:
         h = torch.empty_like(residual if residual.dtype == torch.float32 else x)
-    stats = torch.empty(2 if center else 1, rows, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        rc = lib.gmdn_norm_fwd(_ptr(x), _ptr(residual), _ptr(weight), _ptr(bias), _ptr(y),
-                               _ptr(h), _ptr(stats), _ptr(stats[1] if center else None), rows, D,
-                               eps, center, x.dtype == torch.float32,
-                               residual is not None and residual.dtype == torch.float32, out_f32,
-                               _stream(x))
-    check(rc, "gmdn_norm_fwd")
+    stats = torch.empty((2 if center else 1, rows), dtype=torch.float32, device=x.device)
+    at = stats.data_ptr()
+    _run("gmdn_norm_fwd", lib.gmdn_norm_fwd, x.device, x.data_ptr(), _at(residual), _at(weight),
+         _at(bias), y.data_ptr(), h.data_ptr(), at, at + 4 * rows if center else None, rows, D, eps,
+         center, x.dtype == torch.float32,
+         residual is not None and residual.dtype == torch.float32, out_f32)
     return y, h, stats
 
 
@@ -90,24 +116,20 @@ def _norm_bwd_call(s: Tensor, stats: Tensor, weight: Optional[Tensor], dy: Tenso
     D = s.shape[-1]
     rows = s.numel() // D if D else 0
 
-    def out(wanted, dtype, shape):
-        return torch.empty(shape if wanted else (0,), dtype=dtype, device=s.device)
-
-    da = out(want_bf16, torch.bfloat16, s.shape)
-    db = out(want_f32, torch.float32, s.shape)
-    dweight = out(want_w, torch.float32, (D,))
-    dbias = out(want_b, torch.float32, (D,))
+    none = s.new_empty(0) if not (want_bf16 and want_f32 and want_w and want_b) else None
+    da = torch.empty_like(s, dtype=torch.bfloat16) if want_bf16 else none
+    db = torch.empty_like(s, dtype=torch.float32) if want_f32 else none
+    dweight = stats.new_empty(D) if want_w else none
+    dbias = stats.new_empty(D) if want_b else none
     nbytes = lib.gmdn_norm_bwd_workspace_bytes(rows, D) if want_w or want_b else 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device) if nbytes else None
-    with torch.cuda.device(s.device):
-        rc = lib.gmdn_norm_bwd(_ptr(s), _ptr(stats), _ptr(stats[1] if center else None),
-                               _ptr(weight), _ptr(dy), _ptr(dh), _ptr(da if want_bf16 else None),
-                               _ptr(db if want_f32 else None), _ptr(dweight if want_w else None),
-                               _ptr(dbias if want_b else None), _ptr(ws), nbytes, rows, D, center,
-                               s.dtype == torch.float32, dy.dtype == torch.float32,
-                               dh is not None and dh.dtype == torch.float32, False, True,
-                               _stream(s))
-    check(rc, "gmdn_norm_bwd")
+    at = stats.data_ptr()
+    _run("gmdn_norm_bwd", lib.gmdn_norm_bwd, s.device, s.data_ptr(), at,
+         at + 4 * rows if center else None, _at(weight), dy.data_ptr(), _at(dh),
+         da.data_ptr() if want_bf16 else None, db.data_ptr() if want_f32 else None,
+         dweight.data_ptr() if want_w else None, dbias.data_ptr() if want_b else None, _at(ws),
+         nbytes, rows, D, center, s.dtype == torch.float32, dy.dtype == torch.float32,
+         dh is not None and dh.dtype == torch.float32, False, True)
     return da, db, dweight, dbias
 
 
@@ -131,7 +153,11 @@ def _(x, residual, weight, bias, eps, center, out_f32):
 def _norm_bwd(s: Tensor, stats: Tensor, weight: Optional[Tensor], dy: Tensor,
               dh: Optional[Tensor], center: bool, want_bf16: bool, want_f32: bool, want_w: bool,
               want_b: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
-    return _norm_bwd_call(s, stats, weight, dy, dh, center, want_bf16, want_f32, want_w, want_b)
+    got = _norm_bwd_call(s, stats, weight, dy, dh, center, want_bf16, want_f32, want_w, want_b)
+    wanted = (want_bf16, want_f32, want_w, want_b)
+    types = (torch.bfloat16, torch.float32, torch.float32, torch.float32)
+    # an op's outputs are tensors of their own
+    return tuple(g if w else s.new_empty(0, dtype=t) for g, w, t in zip(got, wanted, types))
 
 
 @_norm_bwd.register_fake
@@ -175,9 +201,13 @@ _norm_fwd.register_autograd(_norm_backward, setup_context=_norm_setup)
 
 
 class _NormFunction(torch.autograd.Function):
-    forward = staticmethod(_norm_fwd_call)
-    setup_context = staticmethod(_norm_setup)
-    backward = staticmethod(once_differentiable(_norm_backward))
+    @staticmethod
+    def forward(ctx, *args):
+        got = _norm_fwd_call(*args)
+        _norm_setup(ctx, args, got)
+        return got
+
+    backward = _once(_norm_backward)
 
 
 def _norm(name: str, center: bool, x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor],
@@ -278,22 +308,17 @@ def _logprobs_fwd_call(logits: Tensor, targets: Optional[Tensor], entropy: bool,
         logits = logits.contiguous()
         rows = _rows_of(logits)
 
-    def out(wanted, size, dtype=torch.float32):
-        return torch.empty(size if wanted else (0,), dtype=dtype, device=logits.device)
-
-    lp = out(targets is not None, shape)
-    ent = out(entropy, shape)
-    tops = out(top_k > 0, (*shape, top_k))
-    ids = out(top_k > 0, (*shape, top_k), torch.int64)
-    stats = torch.empty(*shape, 4, dtype=torch.float32, device=logits.device)
+    stats = torch.empty((*shape, 4), dtype=torch.float32, device=logits.device)
+    lp = stats.new_empty(shape if targets is not None else 0)
+    ent = stats.new_empty(shape if entropy else 0)
+    tops = stats.new_empty((*shape, top_k) if top_k else 0)
+    ids = torch.empty((*shape, top_k) if top_k else 0, dtype=torch.int64, device=logits.device)
     b, t, sb, st = rows
-    with torch.cuda.device(logits.device):
-        rc = lib.gmdn_token_logprobs_fwd(
-            _ptr(logits), _ptr(targets), _ptr(None if targets is None else lp),
-            _ptr(ent if entropy else None), _ptr(tops if top_k else None),
-            _ptr(ids if top_k else None), _ptr(stats), b, t, sb, st, V, top_k, ignore_index,
-            logits.dtype == torch.float32, _stream(logits))
-    check(rc, "gmdn_token_logprobs_fwd")
+    _run("gmdn_token_logprobs_fwd", lib.gmdn_token_logprobs_fwd, logits.device, logits.data_ptr(),
+         _at(targets), lp.data_ptr() if targets is not None else None,
+         ent.data_ptr() if entropy else None, tops.data_ptr() if top_k else None,
+         ids.data_ptr() if top_k else None, stats.data_ptr(), b, t, sb, st, V, top_k, ignore_index,
+         logits.dtype == torch.float32)
     return lp, ent, tops, ids, stats
 
 
@@ -305,13 +330,10 @@ def _logprobs_bwd_call(logits: Tensor, targets: Optional[Tensor], ids: Optional[
         rows = _rows_of(logits)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     b, t, sb, st = rows
-    with torch.cuda.device(logits.device):
-        rc = lib.gmdn_token_logprobs_bwd(
-            _ptr(logits), _ptr(targets), _ptr(stats), _ptr(ids), _ptr(g_lp), _ptr(g_ent),
-            _ptr(g_top), _ptr(grad), b, t, sb, st, logits.shape[-1],
-            0 if g_top is None else g_top.shape[-1], ignore_index,
-            logits.dtype == torch.float32, _stream(logits))
-    check(rc, "gmdn_token_logprobs_bwd")
+    _run("gmdn_token_logprobs_bwd", lib.gmdn_token_logprobs_bwd, logits.device, logits.data_ptr(),
+         _at(targets), stats.data_ptr(), _at(ids), _at(g_lp), _at(g_ent), _at(g_top),
+         grad.data_ptr(), b, t, sb, st, logits.shape[-1], 0 if g_top is None else g_top.shape[-1],
+         ignore_index, logits.dtype == torch.float32)
     return grad
 
 
@@ -367,9 +389,13 @@ _logprobs_fwd.register_autograd(_logprobs_backward, setup_context=_logprobs_setu
 
 
 class _LogprobsFunction(torch.autograd.Function):
-    forward = staticmethod(_logprobs_fwd_call)
-    setup_context = staticmethod(_logprobs_setup)
-    backward = staticmethod(once_differentiable(_logprobs_backward))
+    @staticmethod
+    def forward(ctx, *args):
+        got = _logprobs_fwd_call(*args)
+        _logprobs_setup(ctx, args, got)
+        return got
+
+    backward = _once(_logprobs_backward)
 
 
 def token_logprobs(logits: Tensor, targets: Optional[Tensor] = None, *, entropy: bool = False,
@@ -439,26 +465,21 @@ class Act8Saved(NamedTuple):
 
 
 def _codes_like(x: Tensor) -> tuple[Tensor, Tensor]:
-    return (torch.empty(x.shape, dtype=torch.int8, device=x.device),
+    return (torch.empty_like(x, dtype=torch.int8),
             torch.empty((x.numel() + BLOCK8 - 1) // BLOCK8, dtype=torch.float32, device=x.device))
 
 
 def _pack8_call(x: Tensor) -> tuple[Tensor, Tensor]:
     codes, scales = _codes_like(x)
-    with torch.cuda.device(x.device):
-        rc = lib.gmdn_pack8(_ptr(x), _ptr(codes), _ptr(scales), x.numel(),
-                            x.dtype == torch.float32, _stream(x))
-    check(rc, "gmdn_pack8")
+    _run("gmdn_pack8", lib.gmdn_pack8, x.device, x.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+         x.numel(), x.dtype == torch.float32)
     return codes, scales
 
 
 def _unpack8_call(codes: Tensor, scales: Tensor, f32: bool) -> Tensor:
-    x = torch.empty(codes.shape, dtype=torch.float32 if f32 else torch.bfloat16,
-                    device=codes.device)
-    with torch.cuda.device(codes.device):
-        rc = lib.gmdn_unpack8(_ptr(codes), _ptr(scales), _ptr(x), codes.numel(), f32,
-                              _stream(codes))
-    check(rc, "gmdn_unpack8")
+    x = torch.empty_like(codes, dtype=torch.float32 if f32 else torch.bfloat16)
+    _run("gmdn_unpack8", lib.gmdn_unpack8, codes.device, codes.data_ptr(), scales.data_ptr(),
+         x.data_ptr(), codes.numel(), f32)
     return x
 
 
@@ -470,11 +491,9 @@ def _act8_fwd_call(x: Tensor, gate: Optional[Tensor]) -> tuple[Tensor, Tensor, T
         gcodes, gscales = codes.new_empty(0), scales.new_empty(0)
     else:
         gcodes, gscales = _codes_like(gate)
-    with torch.cuda.device(x.device):
-        rc = lib.gmdn_act8_fwd(_ptr(x), _ptr(gate), _ptr(y), _ptr(codes), _ptr(scales),
-                               _ptr(gcodes), _ptr(gscales), x.numel(), x.dtype == torch.float32,
-                               _stream(x))
-    check(rc, "gmdn_act8_fwd")
+    _run("gmdn_act8_fwd", lib.gmdn_act8_fwd, x.device, x.data_ptr(), _at(gate), y.data_ptr(),
+         codes.data_ptr(), scales.data_ptr(), gcodes.data_ptr(), gscales.data_ptr(), x.numel(),
+         x.dtype == torch.float32)
     return y, codes, scales, gcodes, gscales
 
 
@@ -484,12 +503,10 @@ def _act8_bwd_call(codes: Tensor, scales: Tensor, gcodes: Optional[Tensor],
     dx = torch.empty_like(dy)
     dgate = torch.empty_like(dy) if gcodes is not None else dy.new_empty(0)
     y = torch.empty_like(dy) if restore else dy.new_empty(0)
-    with torch.cuda.device(dy.device):
-        rc = lib.gmdn_act8_bwd(_ptr(codes), _ptr(scales), _ptr(gcodes), _ptr(gscales), _ptr(dy),
-                               _ptr(dx), _ptr(dgate if gcodes is not None else None),
-                               _ptr(y if restore else None), dy.numel(),
-                               dy.dtype == torch.float32, _stream(dy))
-    check(rc, "gmdn_act8_bwd")
+    _run("gmdn_act8_bwd", lib.gmdn_act8_bwd, dy.device, codes.data_ptr(), scales.data_ptr(),
+         _at(gcodes), _at(gscales), dy.data_ptr(), dx.data_ptr(),
+         dgate.data_ptr() if gcodes is not None else None, y.data_ptr() if restore else None,
+         dy.numel(), dy.dtype == torch.float32)
     return dx, dgate, y
 
 
