@@ -517,8 +517,8 @@ static int check_act8(const char* who, std::initializer_list<const void*> ptrs, 
   if (n == 0) return GMDN_OK;
   for (const void* p : ptrs) {
     if (!p) return fail(GMDN_ERR_INVALID, "%s: null pointer", who);
-    if (reinterpret_cast<uintptr_t>(p) % 16)
-      return fail(GMDN_ERR_INVALID, "%s: pointers must be 16-byte aligned", who);
+    if (reinterpret_cast<uintptr_t>(p) % 32)
+      return fail(GMDN_ERR_INVALID, "%s: pointers must be 32-byte aligned", who);
   }
   return GMDN_OK;
 }
@@ -569,8 +569,9 @@ int gmdn_act8_bwd(const int8_t* codes, const float* scales, const int8_t* gate_c
   int rc = check_act8("act8_bwd", {codes, scales, dy, dx}, n);
   if (!rc && gate_codes) rc = check_act8("act8_bwd", {gate_scales, dgate}, n);
   if (rc || n == 0) return rc;
-  if (misaligned({gate_codes, y}))
-    return fail(GMDN_ERR_INVALID, "act8_bwd: pointers must be 16-byte aligned");
+  for (const void* q : {static_cast<const void*>(gate_codes), static_cast<const void*>(y)})
+    if (reinterpret_cast<uintptr_t>(q) % 32)
+      return fail(GMDN_ERR_INVALID, "act8_bwd: pointers must be 32-byte aligned");
   gmdn::Act8Args p{};
   p.codes = const_cast<int8_t*>(codes); p.scales = const_cast<float*>(scales);
   p.gate_codes = const_cast<int8_t*>(gate_codes); p.gate_scales = const_cast<float*>(gate_scales);

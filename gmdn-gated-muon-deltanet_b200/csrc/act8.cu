@@ -26,8 +26,11 @@ namespace {
 constexpr float kTiny = 7.888609052210118e-31f;   // 2^-100
 constexpr float kMagic = 12582912.f;              // 1.5 * 2^23
 constexpr int kWarpsA = 8;
-constexpr int kUnroll = 4;   // blocks (forward) / vectors (backward) a thread has in flight
-constexpr int kCtas = 148 * 8;
+constexpr int kSms = 148;
+// CTAs an SM holds (their registers bound it); the grid is one wave of them
+template <typename T, int kKind>
+constexpr int kResident =
+    (kKind == 0 ? 6 : (kKind == 1 ? 4 : 3)) - (sizeof(T) == 4 ? 1 : 0);
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -40,7 +43,13 @@ __device__ __forceinline__ float rcp(float x) {
   return y;
 }
 
-// tail = P(-|x|) and e = e^(-x^2 / 2) for the type of the tensors.
+// Pairs of elements: two fp32 operations an instruction.
+__device__ __forceinline__ float2 pair(float a) { return make_float2(a, a); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y); }
+
+// P(x) of the normal distribution and e = e^(-x^2 / 2), by the tensors' type.
 //
 // bf16: Abramowitz & Stegun 7.1.26, P(-|x|) = poly(t) e / 2 with
 // t = 1 / (1 + 0.3275911 |x| / sqrt 2): within 0.75e-7 of P (their bound on
@@ -48,301 +57,349 @@ __device__ __forceinline__ float rcp(float x) {
 // two SFU operations and ten others.  fp32: CUDA's normcdff, whose error in
 // ulp the rounding to fp32 needs; those tensors move twice the bytes, which
 // hides its ~3x arithmetic.
+__device__ __forceinline__ void normal2(float2 x, float2& P, float2& e, __nv_bfloat16) {
+  const float2 h = mul2(mul2(x, pair(-0.72134752044448170f)), x);   // -x^2 log2(e) / 2
+  e = make_float2(ex2(h.x), ex2(h.y));
+  const float2 t = make_float2(rcp(fmaf(fabsf(x.x), 0.23164189f, 1.f)),
+                               rcp(fmaf(fabsf(x.y), 0.23164189f, 1.f)));
+  float2 q = fma2(t, pair(0.5307027145f), pair(-0.7265760135f));
+  q = fma2(t, q, pair(0.7107068705f));
+  q = fma2(t, q, pair(-0.142248368f));
+  q = fma2(t, q, pair(0.127414796f));
+  const float2 tail = mul2(mul2(t, q), e);
+  const float2 rest = fma2(tail, pair(-1.f), pair(1.f));
+  P = make_float2(x.x < 0.f ? tail.x : rest.x, x.y < 0.f ? tail.y : rest.y);
+}
+__device__ __forceinline__ void normal2(float2 x, float2& P, float2& e, float) {
+  P = make_float2(normcdff(x.x), normcdff(x.y));
+  e = make_float2(expf(-0.5f * x.x * x.x), expf(-0.5f * x.y * x.y));
+}
+
+__device__ __forceinline__ float2 sigmoid2(float2 a, __nv_bfloat16) {   // within 2^-21
+  const float2 h = mul2(a, pair(-1.4426950408889634f));
+  return make_float2(rcp(1.f + ex2(h.x)), rcp(1.f + ex2(h.y)));
+}
+__device__ __forceinline__ float2 sigmoid2(float2 a, float) {
+  return make_float2(__fdiv_rn(1.f, 1.f + expf(-a.x)), __fdiv_rn(1.f, 1.f + expf(-a.y)));
+}
+
+// 32 bytes (sm_100's widest access), streamed past L1
+struct __align__(32) Wide {
+  uint32_t w[8];
+};
+__device__ __forceinline__ Wide load32(const void* p) {
+  Wide v;
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]),
+                 "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void store32(void* p, const Wide& v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v.w[0]),
+               "r"(v.w[1]), "r"(v.w[2]), "r"(v.w[3]), "r"(v.w[4]), "r"(v.w[5]), "r"(v.w[6]),
+               "r"(v.w[7])
+               : "memory");
+}
+
+// 16 consecutive elements as loaded; an 8th of a block of 128.
+constexpr int kVec = 16;
+constexpr int kLanes = kAct8Block / kVec;   // lanes that share a block
 template <typename T>
-struct Normal;
+struct Vec;
 template <>
-struct Normal<__nv_bfloat16> {
-  __device__ __forceinline__ static void at(float x, float& tail, float& e) {
-    e = ex2(x * x * -0.72134752044448170f);   // -log2(e) / 2
-    const float t = rcp(fmaf(fabsf(x), 0.23164189f, 1.f));
-    float q = fmaf(t, 0.5307027145f, -0.7265760135f);
-    q = fmaf(t, q, 0.7107068705f);
-    q = fmaf(t, q, -0.142248368f);
-    q = fmaf(t, q, 0.127414796f);
-    tail = t * q * e;
+struct Vec<__nv_bfloat16> {
+  Wide r;
+  __device__ __forceinline__ void load(const void* p, uint32_t j) {
+    r = load32(static_cast<const Wide*>(p) + j);
+  }
+  __device__ __forceinline__ float2 get(int k) const {
+    return make_float2(__uint_as_float(r.w[k] << 16), __uint_as_float(r.w[k] & 0xffff0000u));
+  }
+  // the largest magnitude, as fp32 bits: NaN > inf > every number
+  __device__ __forceinline__ uint32_t magnitude() const {
+    uint32_t m = r.w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) m = __vmaxu2(m, r.w[k] & 0x7fff7fffu);
+    return max(m & 0xffff0000u, m << 16);
+  }
+  __device__ __forceinline__ static void store(void* p, uint32_t j, const float2* v) {
+    Wide o;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[k].x, v[k].y);
+      o.w[k] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    store32(static_cast<Wide*>(p) + j, o);
   }
 };
 template <>
-struct Normal<float> {
-  __device__ __forceinline__ static void at(float x, float& tail, float& e) {
-    tail = normcdff(-fabsf(x));
-    e = expf(-0.5f * x * x);
+struct Vec<float> {
+  Wide r[2];
+  __device__ __forceinline__ void load(const void* p, uint32_t j) {
+    r[0] = load32(static_cast<const Wide*>(p) + 2 * static_cast<size_t>(j));
+    r[1] = load32(static_cast<const Wide*>(p) + 2 * static_cast<size_t>(j) + 1);
+  }
+  __device__ __forceinline__ float2 get(int k) const {
+    return make_float2(__uint_as_float(r[k / 4].w[2 * k % 8]),
+                       __uint_as_float(r[k / 4].w[2 * k % 8 + 1]));
+  }
+  __device__ __forceinline__ uint32_t magnitude() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) m = max(m, r[k / 8].w[k % 8] & 0x7fffffffu);
+    return m;
+  }
+  __device__ __forceinline__ static void store(void* p, uint32_t j, const float2* v) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      Wide o;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o.w[2 * k] = __float_as_uint(v[4 * h + k].x);
+        o.w[2 * k + 1] = __float_as_uint(v[4 * h + k].y);
+      }
+      store32(static_cast<Wide*>(p) + 2 * static_cast<size_t>(j) + h, o);
+    }
   }
 };
 
-// P(x) from tail, and from it GELU = x P and its derivative P + x phi.
-__device__ __forceinline__ float share(float x, float tail) { return x < 0.f ? tail : 1.f - tail; }
-
-template <typename T>
-__device__ __forceinline__ float sigmoid(float a);
-template <>
-__device__ __forceinline__ float sigmoid<__nv_bfloat16>(float a) {
-  return rcp(1.f + ex2(a * -1.4426950408889634f));   // within 2^-21
-}
-template <>
-__device__ __forceinline__ float sigmoid<float>(float a) {
-  return __fdiv_rn(1.f, 1.f + expf(-a));
-}
-
-// N consecutive elements (4: 8 or 16 bytes; 8: 16 or 32), aligned
-template <int N>
-__device__ __forceinline__ void load_n(const __nv_bfloat16* p, float* v) {
-  uint32_t r[N / 2];
-  if constexpr (N == 4)
-    *reinterpret_cast<uint2*>(r) = __ldcs(reinterpret_cast<const uint2*>(p));
-  else
-    *reinterpret_cast<uint4*>(r) = __ldcs(reinterpret_cast<const uint4*>(p));
-#pragma unroll
-  for (int k = 0; k < N / 2; ++k) {
-    v[2 * k] = __uint_as_float(r[k] << 16);
-    v[2 * k + 1] = __uint_as_float(r[k] & 0xffff0000u);
-  }
-}
-template <int N>
-__device__ __forceinline__ void load_n(const float* p, float* v) {
-#pragma unroll
-  for (int k = 0; k < N; k += 4)
-    *reinterpret_cast<float4*>(v + k) = __ldcs(reinterpret_cast<const float4*>(p + k));
-}
-template <int N>
-__device__ __forceinline__ void store_n(__nv_bfloat16* p, const float* v) {
-  __nv_bfloat162 r[N / 2];
-#pragma unroll
-  for (int k = 0; k < N / 2; ++k) r[k] = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-  if constexpr (N == 4)
-    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(r);
-  else
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(r);
-}
-template <int N>
-__device__ __forceinline__ void store_n(float* p, const float* v) {
-#pragma unroll
-  for (int k = 0; k < N; k += 4)
-    *reinterpret_cast<float4*>(p + k) = *reinterpret_cast<const float4*>(v + k);
-}
-
-// A block's scale and factor from the largest magnitude of the lane's values
-// (as bits: NaN > inf > every number), one warp a block.
+// A block's scale, and its factor r, from the largest magnitude's bits.
 __device__ __forceinline__ float block_scale(uint32_t top, float& r) {
-  top = __reduce_max_sync(~0u, top);
   const float a = __uint_as_float(top);
   const bool bad = top >= 0x7f800000u, tiny = a < kTiny;
   r = (bad || tiny) ? 0.f : __fdiv_rn(127.f, a);
   return bad ? __int_as_float(0x7fffffff) : (tiny ? 0.f : a * (1.f / 127.f));
 }
-template <int N>
-__device__ __forceinline__ uint32_t magnitude(const float* v) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int k = 0; k < N; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
-  return top;
+// codes of a pair, each in the low byte of its word
+__device__ __forceinline__ float2 code2(float2 v, float r) {
+  return fma2(v, pair(r), pair(kMagic));
 }
-// one element's code in the low byte
-__device__ __forceinline__ uint32_t code(float v, float r) {
-  return __float_as_uint(fmaf(v, r, kMagic));
-}
-__device__ __forceinline__ uint32_t codes4(const float* v, float r) {
-  const uint32_t lo = __byte_perm(code(v[0], r), code(v[1], r), 0x0040);
-  const uint32_t hi = __byte_perm(code(v[2], r), code(v[3], r), 0x0040);
+__device__ __forceinline__ uint32_t codes4(float2 v0, float2 v1, float r) {
+  const float2 a = code2(v0, r), b = code2(v1, r);
+  const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040);
+  const uint32_t hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
   return __byte_perm(lo, hi, 0x5410);
 }
+// the pair that two codes stand for
+__device__ __forceinline__ float2 value2(uint32_t q, int k, float s) {
+  const int a = static_cast<int8_t>(q >> (16 * k)), b = static_cast<int8_t>(q >> (16 * k + 8));
+  return mul2(make_float2(static_cast<float>(a), static_cast<float>(b)), pair(s));
+}
 
-template <typename T, int kKind>   // 0 pack, 1 GELU, 2 SwiGLU
-__device__ __forceinline__ float act_of(float x, float a) {
+template <typename T, int kKind>   // 1 GELU of x, 2 SwiGLU of x and the gate a
+__device__ __forceinline__ float2 act2(float2 x, float2 a) {
   if constexpr (kKind == 1) {
-    float tail, e;
-    Normal<T>::at(x, tail, e);
-    return x * share(x, tail);
+    float2 P, e;
+    normal2(x, P, e, T{});
+    return mul2(x, P);
   } else {
-    return a * sigmoid<T>(a) * x;
+    return mul2(mul2(a, sigmoid2(a, T{})), x);
   }
 }
 
-// One warp a block of 128 elements, 4 consecutive ones a lane; kUnroll blocks
-// loaded before the first is worked on.  One redux gives the block's largest
-// magnitude.
-template <typename T, int kKind>
-__global__ void __launch_bounds__(kWarpsA * 32) act8_fwd_kernel(Act8Args p) {
-  const int lane = threadIdx.x & 31;
-  const long long nw = static_cast<long long>(gridDim.x) * kWarpsA;
-  const long long w = static_cast<long long>(blockIdx.x) * kWarpsA + (threadIdx.x >> 5);
+// The codes and the scale of a lane's 16 elements; 8 lanes (`group`) share a block.
+template <typename T>
+__device__ __forceinline__ void pack_vec(const Vec<T>& v, uint32_t group, uint32_t j,
+                                         int8_t* codes, float* scales) {
+  const uint32_t top = __reduce_max_sync(group, v.magnitude());
+  float r;
+  const float s = block_scale(top, r);
+  uint32_t c[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) c[k] = codes4(v.get(2 * k), v.get(2 * k + 1), r);
+  reinterpret_cast<uint4*>(codes)[j] = make_uint4(c[0], c[1], c[2], c[3]);
+  if (threadIdx.x % kLanes == 0) scales[j / kLanes] = s;
+}
+
+// 16 consecutive elements a lane, a quarter of a warp a block of 128: 32-byte
+// accesses, and one redux and one division for every 16 elements of a lane.
+// The next vector is loaded before the current one is worked on: the kernels
+// are nearly out of instruction slots, so what hides the loads is not more
+// warps.  Vector indexes are 32-bit (the caller splits longer tensors).
+template <typename T, int kKind>   // 0 pack, 1 GELU, 2 SwiGLU
+__global__ void __launch_bounds__(kWarpsA * 32, kResident<T, kKind>) act8_fwd_kernel(Act8Args p) {
+  const uint32_t nt = gridDim.x * blockDim.x;
+  const uint32_t t = blockIdx.x * blockDim.x + threadIdx.x;
+  const uint32_t group = 0xffu << (threadIdx.x & 24);
   const T* x = static_cast<const T*>(p.x);
   const T* gate = static_cast<const T*>(p.gate);
   T* y = static_cast<T*>(p.y);
   const long long full = p.n / kAct8Block;
-  for (long long b0 = w; b0 < full; b0 += nw * kUnroll) {
-    float v[kUnroll][4], a[kKind == 2 ? kUnroll : 1][4];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const long long b = b0 + u * nw;
-      if (b < full) {
-        load_n<4>(x + b * kAct8Block + lane * 4, v[u]);
-        if constexpr (kKind == 2) load_n<4>(gate + b * kAct8Block + lane * 4, a[u]);
-      }
+  const uint32_t vecs = static_cast<uint32_t>(full * kLanes);
+  Vec<T> now, next, gnow, gnext;
+  auto fetch = [&](uint32_t j, Vec<T>& v, Vec<T>& g) {
+    if (j < vecs) {
+      v.load(x, j);
+      if constexpr (kKind == 2) g.load(gate, j);
     }
+  };
+  fetch(t, now, gnow);
+  for (uint32_t j = t; j < vecs; j += nt) {
+    fetch(j + nt, next, gnext);
+    if constexpr (kKind != 0) {
+      float2 out[8];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const long long b = b0 + u * nw;
-      if (b >= full) break;
-      const long long i = b * kAct8Block + lane * 4;
-      if constexpr (kKind != 0) {
-        float out[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          out[k] = act_of<T, kKind>(v[u][k], kKind == 2 ? a[kKind == 2 ? u : 0][k] : 0.f);
-        store_n<4>(y + i, out);
-      }
-      float r;
-      float s = block_scale(magnitude<4>(v[u]), r);
-      *reinterpret_cast<uint32_t*>(p.codes + i) = codes4(v[u], r);
-      if (lane == 0) p.scales[b] = s;
-      if constexpr (kKind == 2) {
-        s = block_scale(magnitude<4>(a[u]), r);
-        *reinterpret_cast<uint32_t*>(p.gate_codes + i) = codes4(a[u], r);
-        if (lane == 0) p.gate_scales[b] = s;
-      }
+      for (int k = 0; k < 8; ++k)
+        out[k] = act2<T, kKind>(now.get(k), kKind == 2 ? gnow.get(k) : now.get(k));
+      Vec<T>::store(y, j, out);
     }
+    pack_vec(now, group, j, p.codes, p.scales);
+    if constexpr (kKind == 2) pack_vec(gnow, group, j, p.gate_codes, p.gate_scales);
+    now = next;
+    if constexpr (kKind == 2) gnow = gnext;
   }
+  // the last, short block: one warp, element lane + 32 k
   const int rest = static_cast<int>(p.n - full * kAct8Block);
-  if (rest == 0 || w != full % nw) return;
-  // the last, short block: element lane + 32 k
+  if (rest == 0 || blockIdx.x != gridDim.x - 1 || threadIdx.x >= 32) return;
   const long long base = full * kAct8Block;
-  float v[4], a[4], r;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int i = lane + 32 * k;
-    v[k] = i < rest ? static_cast<float>(x[base + i]) : 0.f;
-    a[k] = 0.f;
-    if constexpr (kKind == 2)
-      if (i < rest) a[k] = static_cast<float>(gate[base + i]);
-    if constexpr (kKind != 0)
-      if (i < rest) y[base + i] = static_cast<T>(act_of<T, kKind>(v[k], a[k]));
-  }
-  float s = block_scale(magnitude<4>(v), r);
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (lane + 32 * k < rest) p.codes[base + lane + 32 * k] = static_cast<int8_t>(code(v[k], r));
-  if (lane == 0) p.scales[full] = s;
-  if constexpr (kKind == 2) {
-    s = block_scale(magnitude<4>(a), r);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (lane + 32 * k < rest)
-        p.gate_codes[base + lane + 32 * k] = static_cast<int8_t>(code(a[k], r));
-    if (lane == 0) p.gate_scales[full] = s;
-  }
+  const int lane = threadIdx.x;
+  auto pack_rest = [&](const T* in, int8_t* codes, float* scales) {
+    uint32_t top = 0;
+    for (int i = lane; i < rest; i += 32)
+      top = max(top, __float_as_uint(static_cast<float>(in[base + i])) & 0x7fffffffu);
+    float r;
+    const float s = block_scale(__reduce_max_sync(~0u, top), r);
+    for (int i = lane; i < rest; i += 32)
+      codes[base + i] = static_cast<int8_t>(
+          __float_as_uint(fmaf(static_cast<float>(in[base + i]), r, kMagic)));
+    if (lane == 0) scales[full] = s;
+  };
+  pack_rest(x, p.codes, p.scales);
+  if constexpr (kKind == 2) pack_rest(gate, p.gate_codes, p.gate_scales);
+  if constexpr (kKind != 0)
+    for (int i = lane; i < rest; i += 32)
+      y[base + i] = static_cast<T>(
+          act2<T, kKind>(pair(static_cast<float>(x[base + i])),
+                         pair(kKind == 2 ? static_cast<float>(gate[base + i]) : 0.f)).x);
 }
 
-// The backward of one element; kKind 0: the restored value alone.
+// The backward of a pair; kKind 0: the restored value alone.
 template <typename T, int kKind>
-__device__ __forceinline__ void back(float x, float a, float dy, float& dx, float& da, float& y) {
+__device__ __forceinline__ void back2(float2 x, float2 a, float2 dy, float2& dx, float2& da,
+                                      float2& y) {
   if constexpr (kKind == 0) {
     y = x;
   } else if constexpr (kKind == 1) {
-    float tail, e;
-    Normal<T>::at(x, tail, e);
-    const float P = share(x, tail);
-    dx = dy * fmaf(x * 0.3989422804014327f, e, P);
-    y = x * P;
+    float2 P, e;
+    normal2(x, P, e, T{});
+    dx = mul2(dy, fma2(mul2(x, pair(0.3989422804014327f)), e, P));
+    y = mul2(x, P);
   } else {
-    const float sg = sigmoid<T>(a), silu = a * sg;
-    dx = dy * silu;
-    da = dy * x * sg * fmaf(a, 1.f - sg, 1.f);
-    y = silu * x;
+    const float2 sg = sigmoid2(a, T{}), silu = mul2(a, sg);
+    dx = mul2(dy, silu);
+    // sig (1 + a (1 - sig)) = sig + silu - silu sig
+    const float2 slope = fma2(neg2(silu), sg, make_float2(sg.x + silu.x, sg.y + silu.y));
+    da = mul2(mul2(dy, x), slope);
+    y = mul2(silu, x);
   }
 }
 
-// 8 consecutive elements a lane (a 16th of a block), kVecs vectors in flight.
-template <typename T, int kKind>
-__global__ void __launch_bounds__(kWarpsA * 32) act8_bwd_kernel(Act8Args p) {
-  constexpr int kVecs = 2;
-  const long long nt = static_cast<long long>(gridDim.x) * blockDim.x;
-  const long long t = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+template <typename T, int kKind>   // 0 unpack, 1 GELU, 2 SwiGLU
+__global__ void __launch_bounds__(kWarpsA * 32, kResident<T, kKind>) act8_bwd_kernel(Act8Args p) {
+  const uint32_t nt = gridDim.x * blockDim.x;
+  const uint32_t t = blockIdx.x * blockDim.x + threadIdx.x;
   const T* dy = static_cast<const T*>(p.dy);
   T *dx = static_cast<T*>(p.dx), *dg = static_cast<T*>(p.dgate), *y = static_cast<T*>(p.y);
-  const long long vecs = p.n / 8;
-  for (long long j0 = t; j0 < vecs; j0 += nt * kVecs) {
-    uint2 c[kVecs], gc[kKind == 2 ? kVecs : 1];
-    float s[kVecs], gs[kKind == 2 ? kVecs : 1], d[kVecs][8];
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      const long long j = j0 + u * nt;
-      if (j < vecs) {
-        c[u] = __ldcs(reinterpret_cast<const uint2*>(p.codes) + j);
-        s[u] = p.scales[j / (kAct8Block / 8)];
-        if constexpr (kKind == 2) {
-          gc[u] = __ldcs(reinterpret_cast<const uint2*>(p.gate_codes) + j);
-          gs[u] = p.gate_scales[j / (kAct8Block / 8)];
-        }
-        if constexpr (kKind != 0) load_n<8>(dy + j * 8, d[u]);
+  const uint32_t vecs = static_cast<uint32_t>(p.n / kVec);
+  struct In {
+    uint4 c, gc;
+    float s, gs;
+    Vec<T> d;
+  } now, next;
+  auto fetch = [&](uint32_t j, In& in) {
+    if (j < vecs) {
+      in.c = __ldcs(reinterpret_cast<const uint4*>(p.codes) + j);
+      in.s = p.scales[j / kLanes];
+      if constexpr (kKind == 2) {
+        in.gc = __ldcs(reinterpret_cast<const uint4*>(p.gate_codes) + j);
+        in.gs = p.gate_scales[j / kLanes];
       }
+      if constexpr (kKind != 0) in.d.load(dy, j);
     }
+  };
+  auto word = [](const uint4& c, int k) {
+    return k < 2 ? (k < 1 ? c.x : c.y) : (k < 3 ? c.z : c.w);
+  };
+  fetch(t, now);
+  for (uint32_t j = t; j < vecs; j += nt) {
+    fetch(j + nt, next);
+    float2 ox[8], og[8], oy[8];
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u) {
-      const long long j = j0 + u * nt;
-      if (j >= vecs) break;
-      float ox[8], og[8], oy[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int8_t q = static_cast<int8_t>((k < 4 ? c[u].x : c[u].y) >> (8 * (k & 3)));
-        float a = 0.f;
-        if constexpr (kKind == 2)
-          a = static_cast<float>(static_cast<int8_t>((k < 4 ? gc[u].x : gc[u].y) >> (8 * (k & 3)))) *
-              gs[u];
-        back<T, kKind>(static_cast<float>(q) * s[u], a, kKind != 0 ? d[u][k] : 0.f, ox[k], og[k],
-                       oy[k]);
-      }
-      if constexpr (kKind != 0) store_n<8>(dx + j * 8, ox);
-      if constexpr (kKind == 2) store_n<8>(dg + j * 8, og);
-      if (kKind == 0 || y) store_n<8>(y + j * 8, oy);
+    for (int k = 0; k < 8; ++k) {
+      const float2 v = value2(word(now.c, k / 2), k & 1, now.s);
+      float2 a = v, d = v;
+      if constexpr (kKind == 2) a = value2(word(now.gc, k / 2), k & 1, now.gs);
+      if constexpr (kKind != 0) d = now.d.get(k);
+      back2<T, kKind>(v, a, d, ox[k], og[k], oy[k]);
     }
+    if constexpr (kKind != 0) Vec<T>::store(dx, j, ox);
+    if constexpr (kKind == 2) Vec<T>::store(dg, j, og);
+    if (kKind == 0 || y) Vec<T>::store(y, j, oy);
+    now = next;
   }
-  const long long i = vecs * 8 + t;   // the last elements, one a thread
+  const long long i = static_cast<long long>(vecs) * kVec + t;   // the last elements, one a thread
   if (i < p.n) {
-    float a = 0.f, ox, og, oy;
+    float2 a = pair(0.f), ox, og, oy;
     if constexpr (kKind == 2)
-      a = static_cast<float>(p.gate_codes[i]) * p.gate_scales[i / kAct8Block];
-    back<T, kKind>(static_cast<float>(p.codes[i]) * p.scales[i / kAct8Block], a,
-                   kKind != 0 ? static_cast<float>(dy[i]) : 0.f, ox, og, oy);
-    if constexpr (kKind != 0) dx[i] = static_cast<T>(ox);
-    if constexpr (kKind == 2) dg[i] = static_cast<T>(og);
-    if (kKind == 0 || y) y[i] = static_cast<T>(oy);
+      a = pair(static_cast<float>(p.gate_codes[i]) * p.gate_scales[i / kAct8Block]);
+    back2<T, kKind>(pair(static_cast<float>(p.codes[i]) * p.scales[i / kAct8Block]), a,
+                    pair(kKind != 0 ? static_cast<float>(dy[i]) : 0.f), ox, og, oy);
+    if constexpr (kKind != 0) dx[i] = static_cast<T>(ox.x);
+    if constexpr (kKind == 2) dg[i] = static_cast<T>(og.x);
+    if (kKind == 0 || y) y[i] = static_cast<T>(oy.x);
   }
 }
 
-int grid_for(long long units, int per_cta) {
-  const long long want = (units + per_cta - 1) / per_cta;
-  return static_cast<int>(want < 1 ? 1 : (want < kCtas ? want : kCtas));
+// Calls with more elements than the 32-bit vector indexes reach run in slabs.
+constexpr long long kSlab = 1ll << 34;
+
+template <typename T, int kKind, bool kFwd>
+cudaError_t launch(const Act8Args& p, cudaStream_t st) {
+  const long long n = p.n;
+  constexpr size_t es = sizeof(T);
+  constexpr int cap = kSms * kResident<T, kKind>;
+  auto on = [](auto* ptr, size_t bytes) {
+    using P = decltype(ptr);
+    return ptr ? (P)((char*)ptr + bytes) : ptr;
+  };
+  for (long long at = 0; at < n; at += kSlab) {
+    Act8Args q = p;
+    q.n = n - at < kSlab ? n - at : kSlab;
+    q.x = on(p.x, at * es);
+    q.gate = on(p.gate, at * es);
+    q.dy = on(p.dy, at * es);
+    q.dx = on(p.dx, at * es);
+    q.dgate = on(p.dgate, at * es);
+    q.y = on(p.y, at * es);
+    q.codes = on(p.codes, at);
+    q.gate_codes = on(p.gate_codes, at);
+    q.scales = on(p.scales, at / kAct8Block * sizeof(float));
+    q.gate_scales = on(p.gate_scales, at / kAct8Block * sizeof(float));
+    const long long ctas = (q.n + kVec * kWarpsA * 32 - 1) / (kVec * kWarpsA * 32);
+    const int grid = static_cast<int>(ctas < cap ? ctas : cap);
+    if constexpr (kFwd)
+      act8_fwd_kernel<T, kKind><<<grid, kWarpsA * 32, 0, st>>>(q);
+    else
+      act8_bwd_kernel<T, kKind><<<grid, kWarpsA * 32, 0, st>>>(q);
+  }
+  return cudaGetLastError();
 }
 
-template <int kKind>
-cudaError_t fwd(const Act8Args& p, cudaStream_t st) {
-  const int grid = grid_for((p.n + kAct8Block - 1) / kAct8Block, kWarpsA);
-  if (p.f32)
-    act8_fwd_kernel<float, kKind><<<grid, kWarpsA * 32, 0, st>>>(p);
-  else
-    act8_fwd_kernel<__nv_bfloat16, kKind><<<grid, kWarpsA * 32, 0, st>>>(p);
-  return cudaGetLastError();
-}
-template <int kKind>
-cudaError_t bwd(const Act8Args& p, cudaStream_t st) {
-  const int grid = grid_for((p.n + 7) / 8, kWarpsA * 32);
-  if (p.f32)
-    act8_bwd_kernel<float, kKind><<<grid, kWarpsA * 32, 0, st>>>(p);
-  else
-    act8_bwd_kernel<__nv_bfloat16, kKind><<<grid, kWarpsA * 32, 0, st>>>(p);
-  return cudaGetLastError();
+template <int kKind, bool kFwd>
+cudaError_t launch_typed(const Act8Args& p, cudaStream_t st) {
+  return p.f32 ? launch<float, kKind, kFwd>(p, st) : launch<__nv_bfloat16, kKind, kFwd>(p, st);
 }
 
 }  // namespace
 
-cudaError_t pack8(const Act8Args& p, cudaStream_t st) { return fwd<0>(p, st); }
-cudaError_t unpack8(const Act8Args& p, cudaStream_t st) { return bwd<0>(p, st); }
+cudaError_t pack8(const Act8Args& p, cudaStream_t st) { return launch_typed<0, true>(p, st); }
+cudaError_t unpack8(const Act8Args& p, cudaStream_t st) { return launch_typed<0, false>(p, st); }
 cudaError_t act8_fwd(const Act8Args& p, cudaStream_t st) {
-  return p.gated ? fwd<2>(p, st) : fwd<1>(p, st);
+  return p.gated ? launch_typed<2, true>(p, st) : launch_typed<1, true>(p, st);
 }
 cudaError_t act8_bwd(const Act8Args& p, cudaStream_t st) {
-  return p.gated ? bwd<2>(p, st) : bwd<1>(p, st);
+  return p.gated ? launch_typed<2, false>(p, st) : launch_typed<1, false>(p, st);
 }
 
 }  // namespace gmdn

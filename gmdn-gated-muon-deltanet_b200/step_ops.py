@@ -464,6 +464,15 @@ class Act8Saved(NamedTuple):
     gate: Optional[Packed8]
 
 
+def _aligned32(t: Tensor) -> Tensor:
+    """Contiguous and 32-byte aligned, as ``_aligned`` is for 16."""
+    t = _aligned(t)
+    try:
+        return t if t.data_ptr() % 32 == 0 else t.clone()
+    except RuntimeError:   # traced tensors have no storage
+        return t
+
+
 def _codes_like(x: Tensor) -> tuple[Tensor, Tensor]:
     return (torch.empty_like(x, dtype=torch.int8),
             torch.empty((x.numel() + BLOCK8 - 1) // BLOCK8, dtype=torch.float32, device=x.device))
@@ -574,7 +583,7 @@ def pack8(x: Tensor) -> Packed8:
     infinity as NaN.  Not differentiable: the result is a checkpoint."""
     _f32_flag(x, "x")
     _require_cuda("pack8", x)
-    x = _aligned(x.detach())
+    x = _aligned32(x.detach())
     call = _pack8_call if _eager(x) else torch.ops.gmdn.pack8
     return Packed8(*call(x), x.dtype)
 
@@ -583,7 +592,7 @@ def unpack8(packed: Packed8) -> Tensor:
     """The tensor that ``pack8`` kept, in its shape and type."""
     _check_packed("unpack8", packed)
     _same_device("unpack8", packed.codes, packed.scales)
-    codes, scales = _aligned(packed.codes), _aligned(packed.scales)
+    codes, scales = _aligned32(packed.codes), _aligned32(packed.scales)
     call = _unpack8_call if _eager(codes, scales) else torch.ops.gmdn.unpack8
     return call(codes, scales, packed.dtype == torch.float32)
 
@@ -597,7 +606,7 @@ def act8_forward(x: Tensor, gate: Optional[Tensor] = None) -> tuple[Tensor, Act8
         raise ValueError(f"gate must be like x, {tuple(x.shape)} {x.dtype}, got "
                          f"{tuple(gate.shape)} {gate.dtype}")
     _same_device("act8_forward", x, gate)
-    x, gate = _aligned(x.detach()), None if gate is None else _aligned(gate.detach())
+    x, gate = _aligned32(x.detach()), None if gate is None else _aligned32(gate.detach())
     call = _act8_fwd_call if _eager(x, gate) else torch.ops.gmdn.act8_fwd
     y, codes, scales, gcodes, gscales = call(x, gate)
     return y, Act8Saved(Packed8(codes, scales, x.dtype),
@@ -620,8 +629,8 @@ def act8_backward(saved: Act8Saved, dy: Tensor, restore: bool = True):
             raise ValueError("act8_backward: the gate's checkpoint is not like the input's")
     parts = [x.codes, x.scales] + ([None, None] if gate is None else [gate.codes, gate.scales])
     _same_device("act8_backward", dy, *parts)
-    parts = [None if t is None else _aligned(t) for t in parts]
-    dy = _aligned(dy.detach())
+    parts = [None if t is None else _aligned32(t) for t in parts]
+    dy = _aligned32(dy.detach())
     call = _act8_bwd_call if _eager(dy, *parts) else torch.ops.gmdn.act8_bwd
     dx, dgate, y = call(*parts, dy, bool(restore))
     return dx, dgate if gate is not None else None, y if restore else None

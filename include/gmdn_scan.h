@@ -287,7 +287,7 @@ int gmdn_token_logprobs_bwd(const void* logits, const int64_t* targets, const fl
  * code * fp32(a * fp32(1 / 127)): off by at most half a step a / 254 and
  * rounding.  Blocks with a < 2^-100 come back as zeros, blocks with a NaN or an
  * infinity as NaN.  codes n bytes, scales ceil(n / 128) fp32; all pointers
- * 16-byte aligned.  No counterpart in the reference. */
+ * 32-byte aligned.  No counterpart in the reference. */
 int gmdn_pack8(const void* x, int8_t* codes, float* scales, long long n, int f32, void* stream);
 int gmdn_unpack8(const int8_t* codes, const float* scales, void* x, long long n, int f32,
                  void* stream);
