@@ -452,7 +452,7 @@ static int check_logprobs(const void* logits, long long batch, long long length,
   if (batch < 0 || length < 0 || vocab < 1)
     return fail(GMDN_ERR_INVALID, "token_logprobs: bad size batch=%lld length=%lld vocab=%d", batch,
                 length, vocab);
-  if (length > 0 && batch > (1ll << 60) / length / vocab)
+  if (vocab > (1 << 30) || (length > 0 && batch > (1ll << 60) / length / vocab))
     return fail(GMDN_ERR_UNSUPPORTED, "token_logprobs: too many elements");
   if (top_k < 0 || top_k > gmdn::kMaxTopK || top_k > vocab)
     return fail(GMDN_ERR_INVALID, "token_logprobs: top_k must be in [0, min(%d, vocab)] (got %d)",

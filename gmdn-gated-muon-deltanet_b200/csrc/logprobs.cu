@@ -17,8 +17,19 @@
 // -inf, entropy 0 and no gradient; a row with a NaN or +inf gives NaN.
 //
 // Alternatives are the top_k largest logits, ties to the lowest index; in a
-// NaN row every column ties.
+// NaN row every column ties.  They come out of the same pass: a thread's own
+// maximum is at hand when it is over, the top_k-th largest of 128 maxima (of
+// groups of threads) is a bound that at least top_k columns reach and about
+// top_k more do not pass, and only the threads whose maximum reaches it read
+// their columns again (from L2).
+//
+// A row is read by one CTA, or, where there are fewer rows than SMs, by a
+// cluster of up to 8 whose parts are joined over distributed shared memory.
+// Rows may start at any alignment: a thread works on whole 16-byte chunks of
+// the address space, and the first and the last chunk of a row element by
+// element.
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <float.h>
@@ -29,42 +40,113 @@
 namespace gmdn {
 namespace {
 
-constexpr int kLpThreads = 512;
+namespace cg = cooperative_groups;
+using bf16 = __nv_bfloat16;
+
+constexpr int kSms = 148;
+constexpr int kMaxThreads = 512;
+constexpr int kMaxCluster = 8;
+constexpr int kGroups = 128;   // maxima the bound is taken from
+constexpr int kList = 1024;    // columns above the bound, or at it, that are kept
+static_assert(kList >= kMaxCluster * kMaxTopK, "rank 0 joins the cluster's lists in one");
 // Logarithms are clamped here where they multiply a factor e^c: that is 0 long
 // before, and 0 * -inf, or a sum of S times a mask's -3e38, is not a number.
 constexpr float kFar = -1000.f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 pair(float a) { return make_float2(a, a); }
 
 struct Stat {
   float m, s, q;
 };
-
-__device__ __forceinline__ void join(Stat& a, float m, float s, float q) {
-  const float mn = fmaxf(a.m, m);
-  const float da = fmaxf(a.m - mn, kFar), db = fmaxf(m - mn, kFar);
-  const float fa = __expf(da), fb = __expf(db);
-  a.q = fa * fmaf(a.s, da, a.q) + fb * fmaf(s, db, q);
-  a.s = fa * a.s + fb * s;
+__device__ __forceinline__ void join(Stat& a, const Stat& b) {
+  const float mn = fmaxf(a.m, b.m);
+  const float da = fmaxf(a.m - mn, kFar), db = fmaxf(b.m - mn, kFar);
+  const float fa = ex2(da * kLog2e), fb = ex2(db * kLog2e);
+  a.q = fa * fmaf(a.s, da, a.q) + fb * fmaf(b.s, db, b.q);
+  a.s = fa * a.s + fb * b.s;
   a.m = mn;
 }
 
-__device__ __forceinline__ void add(Stat& a, float x) {
-  if (x > a.m) {
-    const float d = fmaxf(a.m - x, kFar);
-    const float f = __expf(d);
-    a.q = f * fmaf(a.s, d, a.q);
-    a.s *= f;
-    a.m = x;
+// 16 bytes of a row
+template <typename T>
+struct Chunk;
+template <>
+struct Chunk<bf16> {
+  static constexpr int E = 8;
+  uint32_t w[4];
+  __device__ __forceinline__ float2 get(int k) const {
+    return make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
   }
-  const float c = x - a.m;
-  const float e = __expf(c);   // NaN stays NaN in s
-  a.s += e;
-  a.q = fmaf(e, fmaxf(c, kFar), a.q);
+  __device__ __forceinline__ void set(int i, float v) {   // i constant after unrolling
+    const uint32_t b = f32_to_bf16(v);
+    w[i / 2] = i & 1 ? (w[i / 2] & 0xffffu) | (b << 16) : (w[i / 2] & 0xffff0000u) | b;
+  }
+  __device__ __forceinline__ float largest() const {   // NaN left out
+    __nv_bfloat162 h[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h[k] = *reinterpret_cast<const __nv_bfloat162*>(&w[k]);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+};
+template <>
+struct Chunk<float> {
+  static constexpr int E = 4;
+  uint32_t w[4];
+  __device__ __forceinline__ float2 get(int k) const {
+    return make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+  }
+  __device__ __forceinline__ void set(int i, float v) { w[i] = __float_as_uint(v); }
+  __device__ __forceinline__ float largest() const {
+    return fmaxf(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])),
+                 fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3])));
+  }
+};
+template <typename T>
+__device__ __forceinline__ float value(const Chunk<T>& c, int i) {
+  const float2 v = c.get(i / 2);
+  return i & 1 ? v.y : v.x;
+}
+template <typename T>
+__device__ __forceinline__ float element(const T* p) {
+  return static_cast<float>(*p);
 }
 
-__device__ __forceinline__ const char* row_of(const LogprobArgs& p, long long r) {
-  const long long b = r / p.length, t = r - b * p.length;
-  return static_cast<const char*>(p.logits) + (b * p.stride_b + t * p.stride_t) * (p.f32 ? 4 : 2);
-}
+// A row as chunks: chunk j holds elements first(j) .. first(j) + E - 1, those
+// outside the row read as -inf.
+template <typename T>
+struct Row {
+  static constexpr int E = Chunk<T>::E;
+  const T* x;
+  int V, off, chunks;
+  __device__ __forceinline__ Row(const T* row, int vocab) : x(row), V(vocab) {
+    off = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
+    chunks = (off + V - 1) / E + 1;
+  }
+  __device__ __forceinline__ int first(int j) const { return j * E - off; }
+  __device__ __forceinline__ Chunk<T> load(int j) const {
+    const int i0 = first(j);
+    Chunk<T> c;
+    if (i0 >= 0 && i0 <= V - E) {
+      const uint4 r = __ldg(reinterpret_cast<const uint4*>(x + i0));
+      c.w[0] = r.x;
+      c.w[1] = r.y;
+      c.w[2] = r.z;
+      c.w[3] = r.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        c.set(k, i0 + k >= 0 && i0 + k < V ? element(x + i0 + k) : -INFINITY);
+    }
+    return c;
+  }
+};
 
 // (value, index) in one key: larger value first, then the lower index.
 __device__ __forceinline__ unsigned long long key_of(float v, int i) {
@@ -72,63 +154,95 @@ __device__ __forceinline__ unsigned long long key_of(float v, int i) {
   u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
   return (static_cast<unsigned long long>(u) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
 }
+__device__ __forceinline__ int key_index(unsigned long long k) {
+  return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k));
+}
+__device__ __forceinline__ float key_value(unsigned long long k) {
+  const uint32_t u = static_cast<uint32_t>(k >> 32);
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
 
-__global__ void __launch_bounds__(kLpThreads) logprobs_fwd_rows(LogprobArgs p, long long rows) {
-  __shared__ float sm[32], ss[32], sq[32];
-  __shared__ unsigned long long best[32];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const char* row = row_of(p, r);
-    Stat a{-FLT_MAX, 0.f, 0.f};
-    for (int j = threadIdx.x; j < p.vocab; j += kLpThreads) add(a, load_act(row, j, p.f32));
+struct TopShared {
+  unsigned long long above[kList], at[kList];
+  unsigned long long best[kMaxTopK];
+  float thread_max[kMaxThreads], group_max[kGroups];
+  unsigned long long warp_best[kMaxThreads / 32];
+  int warp_count[kMaxThreads / 32];
+  int n_above, n_at, have;
+  float bound;
+};
+
+// The place of key i among n keys, largest first.
+__device__ __forceinline__ int place(const unsigned long long* keys, int n, unsigned long long k) {
+  int r = 0;
+  for (int i = 0; i < n; ++i) r += keys[i] > k;
+  return r;
+}
+
+// The min(k, columns) largest columns of chunks [c0, c1) into sh.best, falling;
+// `mine`: the thread's largest value (at least -FLT_MAX) over chunks c0 + tid,
+// + blockDim, ....  No NaN among them.
+template <typename T>
+__device__ void top_columns(TopShared& sh, const Row<T>& row, int c0, int c1, int k, float mine) {
+  constexpr int E = Chunk<T>::E;
+  const int tid = threadIdx.x, n = blockDim.x, lane = tid & 31, w = tid >> 5;
+  sh.thread_max[tid] = mine;
+  if (tid == 0) sh.n_above = sh.n_at = 0;
+  __syncthreads();
+  if (tid < kGroups) {
+    // groups of threads far apart: chunks that lie together fall into different groups
+    float g = mine;
+    for (int t = tid + kGroups; t < n; t += kGroups) g = fmaxf(g, sh.thread_max[t]);
+    sh.group_max[tid] = g;
+  }
+  __syncthreads();
+  if (tid < kGroups) {
+    const float g = sh.group_max[tid];
+    int r = 0;
+#pragma unroll 8
+    for (int t = 0; t < kGroups; ++t) {
+      const float o = sh.group_max[t];
+      r += o > g || (o == g && t < tid);
+    }
+    if (r == k - 1) sh.bound = g;
+  }
+  __syncthreads();
+  const float bound = sh.bound;
+  const int lo = max(row.first(c0), 0), hi = min(row.first(c1), row.V);
+  const int want = max(min(k, hi - lo), 0);
+  if (mine >= bound) {
+    for (int j = c0 + tid; j < c1; j += n) {
+      const Chunk<T> c = row.load(j);
+      if (!(c.largest() >= bound)) continue;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-      join(a, __shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o),
-           __shfl_xor_sync(~0u, a.q, o));
-    if (lane == 0) {
-      sm[w] = a.m;
-      ss[w] = a.s;
-      sq[w] = a.q;
-    }
-    __syncthreads();
-    a = Stat{sm[0], ss[0], sq[0]};
-    for (int k = 1; k < kLpThreads / 32; ++k) join(a, sm[k], ss[k], sq[k]);
-    const bool empty = a.s == 0.f, bad = !(a.s >= 0.f) || a.m == INFINITY;
-    const float ls = logf(a.s);
-    const float nan = __int_as_float(0x7fffffff);
-    auto logprob = [&](float x) {
-      return bad ? nan : (empty ? -INFINITY : (x - a.m) - ls);
-    };
-    if (threadIdx.x == 0) {
-      const float H = bad ? nan : (empty ? 0.f : ls - a.q / a.s);
-      if (p.stats) {
-        float4 st = make_float4(a.m, ls, H, 0.f);
-        if (bad) st.y = nan;
-        reinterpret_cast<float4*>(p.stats)[r] = st;
-      }
-      if (p.entropy) p.entropy[r] = H;
-      if (p.logprobs) {
-        const int64_t t = p.targets[r];
-        float lp = 0.f;
-        if (t != p.ignore_index)
-          lp = (t >= 0 && t < p.vocab) ? logprob(load_act(row, t, p.f32)) : nan;
-        p.logprobs[r] = lp;
-      }
-    }
-    // alternatives: k rounds, each the largest key below the last one taken
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < p.top_k; ++k) {
-      if (bad) {
-        if (threadIdx.x == 0) {
-          p.top_ids[r * p.top_k + k] = k;
-          p.top_logprobs[r * p.top_k + k] = nan;
+      for (int e = 0; e < E; ++e) {
+        const float v = value(c, e);
+        const int i = row.first(j) + e;
+        if (v >= bound && i >= 0 && i < row.V) {
+          int* count = v > bound ? &sh.n_above : &sh.n_at;
+          unsigned long long* list = v > bound ? sh.above : sh.at;
+          const int slot = atomicAdd(count, 1);
+          if (slot < kList) list[slot] = key_of(v, i);
         }
-        continue;
       }
+    }
+  }
+  __syncthreads();
+  const int na = sh.n_above, nt = sh.n_at;
+  if (na > kList) {
+    // more columns above the bound than the list holds (they all lie in few threads): one
+    // column a round, the largest below the last
+    unsigned long long last = ~0ull;
+    for (int r = 0; r < want; ++r) {
       unsigned long long b = 0;
-      for (int j = threadIdx.x; j < p.vocab; j += kLpThreads) {
-        const unsigned long long q = key_of(load_act(row, j, p.f32), j);
-        if (q < last && q > b) b = q;
+      for (int j = c0 + tid; j < c1; j += n) {
+        const Chunk<T> c = row.load(j);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int i = row.first(j) + e;
+          const unsigned long long q = key_of(value(c, e), i);
+          if (i >= 0 && i < row.V && q < last && q > b) b = q;
+        }
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
@@ -136,78 +250,412 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_fwd_rows(LogprobArgs p, l
         if (q > b) b = q;
       }
       __syncthreads();
-      if (lane == 0) best[w] = b;
+      if (lane == 0) sh.warp_best[w] = b;
       __syncthreads();
-      for (int i = 0; i < kLpThreads / 32; ++i)
-        if (best[i] > b) b = best[i];
+      for (int i = 0; i < n / 32; ++i)
+        if (sh.warp_best[i] > b) b = sh.warp_best[i];
       last = b;
-      if (threadIdx.x == 0) {
-        const int id = static_cast<int>(0xffffffffu - static_cast<uint32_t>(b));
-        p.top_ids[r * p.top_k + k] = id;
-        p.top_logprobs[r * p.top_k + k] = logprob(load_act(row, id, p.f32));
-      }
+      if (tid == 0) sh.best[r] = b;
     }
     __syncthreads();
+    if (tid == 0) sh.have = want;
+    __syncthreads();
+    return;
+  }
+  for (int i = tid; i < na; i += n) {
+    const int r = place(sh.above, na, sh.above[i]);
+    if (r < want) sh.best[r] = sh.above[i];
+  }
+  int have = min(na, want);
+  if (have < want && nt <= kList) {
+    for (int i = tid; i < nt; i += n) {
+      const int r = na + place(sh.at, nt, sh.at[i]);
+      if (r < want) sh.best[r] = sh.at[i];
+    }
+    have = min(na + nt, want);
+  }
+  // Too many columns at the bound to list, or (bound -FLT_MAX) columns at -inf are needed too:
+  // the first ones in order, tile by tile.
+  float tie = nt <= kList ? -INFINITY : bound;
+  for (int pass = 0; pass < 2 && have < want; ++pass) {
+    int found = 0;
+    for (int base = c0; base < c1 && have + found < want; base += n) {
+      const int j = base + tid;
+      uint32_t hits = 0;
+      if (j < c1) {
+        const Chunk<T> c = row.load(j);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int i = row.first(j) + e;
+          if (value(c, e) == tie && i >= 0 && i < row.V) hits |= 1u << e;
+        }
+      }
+      const int mine_n = __popc(hits);
+      int before = mine_n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(~0u, before, o);
+        if (lane >= o) before += v;
+      }
+      __syncthreads();
+      if (lane == 31) sh.warp_count[w] = before;
+      __syncthreads();
+      before -= mine_n;
+      int total = 0;
+      for (int i = 0; i < n / 32; ++i) {
+        if (i < w) before += sh.warp_count[i];
+        total += sh.warp_count[i];
+      }
+      for (int e = 0; e < E; ++e)
+        if (hits >> e & 1) {
+          const int r = have + found + before++;
+          if (r < want) sh.best[r] = key_of(tie, row.first(j) + e);
+        }
+      found += total;
+    }
+    have = min(have + found, want);
+    tie = -INFINITY;   // below the lowest finite value there is nothing else
+  }
+  if (tid == 0) sh.have = want;
+  __syncthreads();
+}
+
+// Max, sum and (kEnt) entropy sum of U chunks.
+template <typename T, bool kEnt, int U>
+__device__ __forceinline__ void absorb(const Chunk<T>* c, float& m, float2& s, float2& q) {
+  constexpr int P = Chunk<T>::E / 2;
+  float top = c[0].largest();
+#pragma unroll
+  for (int u = 1; u < U; ++u) top = fmaxf(top, c[u].largest());
+  if (top > m) {
+    const float d = fmaxf(m - top, kFar), f = ex2(d * kLog2e);
+    if constexpr (kEnt) {
+      q.x = f * fmaf(s.x, d, q.x);
+      q.y = f * fmaf(s.y, d, q.y);
+    }
+    s = __fmul2_rn(s, pair(f));
+    m = top;
+  }
+  const float2 nm = pair(-m);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      float2 d = __fadd2_rn(c[u].get(k), nm);
+      const float2 y = __fmul2_rn(d, pair(kLog2e));
+      const float2 e = make_float2(ex2(y.x), ex2(y.y));   // NaN stays
+      s = __fadd2_rn(s, e);
+      if constexpr (kEnt) {
+        d = make_float2(fmaxf(d.x, kFar), fmaxf(d.y, kFar));
+        q = __ffma2_rn(e, d, q);
+      }
+    }
+}
+
+constexpr int kUnroll = 4;
+
+template <typename T, bool kEnt, bool kTop, bool kCluster>
+__global__ void __launch_bounds__(kMaxThreads) logprobs_fwd_kernel(LogprobArgs p) {
+  extern __shared__ __align__(16) char dyn[];   // kTop: TopShared
+  __shared__ Stat warp_stat[kMaxThreads / 32];
+  __shared__ Stat cta_stat;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, n = blockDim.x;
+  int parts = 1, rank = 0;
+  if constexpr (kCluster) {
+    parts = cg::this_cluster().num_blocks();
+    rank = cg::this_cluster().block_rank();
+  }
+  const long long r = blockIdx.x / parts;
+  const long long b = r / p.length;
+  const T* x = static_cast<const T*>(p.logits) + b * p.stride_b + (r - b * p.length) * p.stride_t;
+  const Row<T> row(x, p.vocab);
+  // the given token's logit, on its way while the row is read
+  const bool writer = rank == 0 && tid == 0;
+  int64_t t = 0;
+  float xt = 0.f;
+  if (writer && p.logprobs) {
+    t = p.targets[r];
+    if (t >= 0 && t < p.vocab) xt = element(x + t);
+  }
+  const int per = (row.chunks + parts - 1) / parts;
+  const int c0 = min(rank * per, row.chunks), c1 = min(c0 + per, row.chunks);
+  float m = -FLT_MAX;
+  float2 s = pair(0.f), q = pair(0.f);
+  int j = c0 + tid;
+  for (; j + (kUnroll - 1) * n < c1; j += kUnroll * n) {
+    Chunk<T> c[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) c[u] = row.load(j + u * n);
+    absorb<T, kEnt, kUnroll>(c, m, s, q);
+  }
+  for (; j < c1; j += n) {
+    const Chunk<T> c = row.load(j);
+    absorb<T, kEnt, 1>(&c, m, s, q);
+  }
+  const float mine = m;
+  Stat a{m, s.x + s.y, q.x + q.y};
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    join(a, Stat{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o),
+                 __shfl_xor_sync(~0u, a.q, o)});
+  if (lane == 0) warp_stat[w] = a;
+  __syncthreads();
+  a = warp_stat[0];
+  for (int k = 1; k < n / 32; ++k) join(a, warp_stat[k]);
+  if constexpr (kCluster) {
+    auto cluster = cg::this_cluster();
+    if (tid == 0) cta_stat = a;
+    cluster.sync();
+    a = *cluster.map_shared_rank(&cta_stat, 0);
+    for (int k = 1; k < parts; ++k) join(a, *cluster.map_shared_rank(&cta_stat, k));
+  }
+  const bool empty = a.s == 0.f, bad = !(a.s >= 0.f) || a.m == INFINITY;
+  const float ls = logf(a.s), nan = __int_as_float(0x7fffffff);
+  auto logprob = [&](float v) { return bad ? nan : (empty ? -INFINITY : (v - a.m) - ls); };
+  if (writer) {
+    const float H = bad ? nan : (empty ? 0.f : ls - a.q / a.s);
+    if (p.stats)
+      reinterpret_cast<float4*>(p.stats)[r] = make_float4(a.m, bad ? nan : ls, kEnt ? H : nan, 0.f);
+    if (p.entropy) p.entropy[r] = H;
+    if (p.logprobs)
+      p.logprobs[r] = t == p.ignore_index ? 0.f : (t >= 0 && t < p.vocab ? logprob(xt) : nan);
+  }
+  if constexpr (kTop) {
+    TopShared& sh = *reinterpret_cast<TopShared*>(dyn);
+    if (!bad) top_columns(sh, row, c0, c1, p.top_k, mine);
+    if constexpr (kCluster) {
+      // rank 0 takes the cluster's lists together
+      auto cluster = cg::this_cluster();
+      cluster.sync();
+      if (rank == 0 && !bad) {
+        int have = 0;
+        for (int k = 0; k < parts; ++k) {
+          const TopShared* other = cluster.map_shared_rank(&sh, k);
+          const int nk = other->have;
+          for (int i = tid; i < nk; i += n) sh.above[have + i] = other->best[i];
+          have += nk;
+        }
+        __syncthreads();
+        for (int i = tid; i < have; i += n) {
+          const int at = place(sh.above, have, sh.above[i]);
+          if (at < p.top_k) sh.best[at] = sh.above[i];
+        }
+        __syncthreads();
+      }
+      cluster.sync();   // the others' shared memory is read until here
+    }
+    if (rank == 0 && tid < p.top_k) {
+      const long long o = r * p.top_k + tid;
+      p.top_ids[o] = bad ? tid : key_index(sh.best[tid]);
+      p.top_logprobs[o] = bad ? nan : logprob(key_value(sh.best[tid]));
+    }
+  } else if constexpr (kCluster) {
+    cg::this_cluster().sync();
   }
 }
 
-// The gradient of column x of a row, without the terms of given columns.
-struct RowGrad {
-  float m, ls, H, w, gh;   // w = gl + sum gk
-  bool empty;
-  __device__ __forceinline__ float at(float x) const {
-    if (empty) return 0.f;
-    const float lp = fmaxf((x - m) - ls, kFar);
-    // a masked column: p = 0, no gradient; NaN stays
-    const float pr = __expf((x - m) - ls);
-    return -pr * fmaf(gh, lp + H, w);
-  }
-};
+// ---------------------------------------------------------------------------
+// gradient
+// ---------------------------------------------------------------------------
 
-__global__ void __launch_bounds__(kLpThreads) logprobs_bwd_rows(LogprobArgs p, long long rows) {
-  const size_t es = p.f32 ? 4 : 2;
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const char* row = row_of(p, r);
-    char* out = static_cast<char*>(p.dlogits) + static_cast<size_t>(r) * p.vocab * es;
-    const float4 st = reinterpret_cast<const float4*>(p.stats)[r];
-    RowGrad g{st.x, st.y, st.z, 0.f, p.g_entropy ? p.g_entropy[r] : 0.f, st.y == -INFINITY};
-    int64_t t = -1;
-    float gl = 0.f;
-    if (p.g_logprobs && p.targets[r] != p.ignore_index) {
-      t = p.targets[r];
-      gl = (t >= 0 && t < p.vocab) ? p.g_logprobs[r] : __int_as_float(0x7fffffff);
-      if (t >= p.vocab) t = -1;
-    }
-    g.w = gl;
-    if (p.g_top)
-      for (int k = 0; k < p.top_k; ++k) g.w += p.g_top[r * p.top_k + k];
-    for (int j = threadIdx.x; j < p.vocab; j += kLpThreads) {
-      float v = g.at(load_act(row, j, p.f32));
-      if (!g.empty) {
-        if (j == t) v += gl;
-        if (p.g_top)
-          for (int k = 0; k < p.top_k; ++k)
-            if (p.top_ids[r * p.top_k + k] == j) v += p.g_top[r * p.top_k + k];
-      }
-      store_act(out, j, v, p.f32);
+constexpr int kBwdThreads = 256;
+
+// Elements i0 .. i0 + E - 1 of a row that lies `shift` elements above a 16-byte
+// boundary there: the two aligned chunks that hold them, shifted together.
+template <typename T>
+__device__ __forceinline__ Chunk<T> load_shifted(const T* x, int i0, int shift) {
+  Chunk<T> c;
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(x + i0 - shift));
+  if (shift == 0) {
+    c.w[0] = a.x;
+    c.w[1] = a.y;
+    c.w[2] = a.z;
+    c.w[3] = a.w;
+    return c;
+  }
+  const uint4 b = __ldg(reinterpret_cast<const uint4*>(x + i0 - shift) + 1);
+  uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  const int bytes = shift * static_cast<int>(sizeof(T));
+  if (bytes & 8) {
+#pragma unroll
+    for (int k = 0; k < 6; ++k) v[k] = v[k + 2];
+  }
+  if (bytes & 4) {
+#pragma unroll
+    for (int k = 0; k < 5; ++k) v[k] = v[k + 1];
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) c.w[k] = bytes & 2 ? __funnelshift_r(v[k], v[k + 1], 16) : v[k];
+  return c;
+}
+
+// Grid: `parts` CTAs a row.  The gradient of a column is p (A + B logprob),
+// A = -(w + gH H), B = -gH, w = gl + sum gk; the given token's column has gl
+// on top where it is computed, the alternatives' columns are written again at
+// the end, each by one thread.
+template <typename T, bool kEnt, bool kTop>
+__global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p, int parts) {
+  constexpr int E = Chunk<T>::E, U = 4;
+  const long long r = blockIdx.x / parts;
+  const int part = static_cast<int>(blockIdx.x - r * parts), tid = threadIdx.x, n = blockDim.x;
+  const long long b = r / p.length;
+  const T* x = static_cast<const T*>(p.logits) + b * p.stride_b + (r - b * p.length) * p.stride_t;
+  T* out = static_cast<T*>(p.dlogits) + r * p.vocab;
+  const int V = p.vocab;
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(out) % 16 / sizeof(T));
+  const int chunks = (off + V - 1) / E + 1;
+  // every chunk of `out` starts `shift` elements above a boundary of the logits
+  const int shift =
+      static_cast<int>((reinterpret_cast<uintptr_t>(x) / sizeof(T) + E - off) % E);
+  const int c0 = part * n * U;
+  auto load = [&](int j) {
+    const int i0 = j * E - off;
+    if (i0 - shift >= 0 && i0 - shift + (shift ? 2 * E : E) <= V) return load_shifted(x, i0, shift);
+    Chunk<T> c;
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+      c.set(k, i0 + k >= 0 && i0 + k < V ? element(x + i0 + k) : -INFINITY);
+    return c;
+  };
+  Chunk<T> c[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (c0 + u * n + tid < chunks) c[u] = load(c0 + u * n + tid);
+  const float4 st = __ldg(reinterpret_cast<const float4*>(p.stats) + r);
+  const float m = st.x, ls = st.y, nan = __int_as_float(0x7fffffff);
+  const bool empty = ls == -INFINITY;
+  const float gh = kEnt && p.g_entropy ? p.g_entropy[r] : 0.f;
+  int t = -1;
+  float gl = 0.f;
+  if (p.g_logprobs) {
+    const int64_t tt = p.targets[r];
+    if (tt != p.ignore_index) {
+      const bool ok = tt >= 0 && tt < V;
+      gl = ok ? p.g_logprobs[r] : nan;
+      t = ok ? static_cast<int>(tt) : -1;
     }
   }
+  float wsum = gl;
+  if constexpr (kTop)
+    for (int k = 0; k < p.top_k; ++k) wsum += p.g_top[r * p.top_k + k];
+  const float A = kEnt ? -fmaf(gh, st.z, wsum) : -wsum, B = -gh;
+  auto grad2 = [&](float2 v) {
+    float2 lp = __fadd2_rn(__fadd2_rn(v, pair(-m)), pair(-ls));
+    const float2 y = __fmul2_rn(lp, pair(kLog2e));
+    const float2 e = make_float2(ex2(y.x), ex2(y.y));
+    if constexpr (kEnt) {
+      lp = make_float2(fmaxf(lp.x, kFar), fmaxf(lp.y, kFar));
+      return __fmul2_rn(e, __ffma2_rn(lp, pair(B), pair(A)));
+    }
+    return __fmul2_rn(e, pair(A));
+  };
+  const int tj = t >= 0 ? (t + off) / E : -1;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int j = c0 + u * n + tid;
+    if (j >= chunks) break;
+    float2 g[E / 2];
+#pragma unroll
+    for (int k = 0; k < E / 2; ++k) g[k] = empty ? pair(0.f) : grad2(c[u].get(k));
+    const int i0 = j * E - off;
+    if (j == tj && !empty) {
+#pragma unroll
+      for (int k = 0; k < E / 2; ++k) {
+        if (i0 + 2 * k == t) g[k].x += gl;
+        if (i0 + 2 * k + 1 == t) g[k].y += gl;
+      }
+    }
+    if (i0 >= 0 && i0 + E <= V) {
+      uint4 o;
+      if constexpr (sizeof(T) == 2) {
+        __nv_bfloat162 h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = __floats2bfloat162_rn(g[k].x, g[k].y);
+        o = *reinterpret_cast<uint4*>(h);
+      } else {
+        o = make_uint4(__float_as_uint(g[0].x), __float_as_uint(g[0].y), __float_as_uint(g[1].x),
+                       __float_as_uint(g[1].y));
+      }
+      *reinterpret_cast<uint4*>(out + i0) = o;
+    } else {
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if (i0 + k >= 0 && i0 + k < V)
+          out[i0 + k] = static_cast<T>(k & 1 ? g[k / 2].y : g[k / 2].x);
+    }
+  }
+  if constexpr (kTop) {
+    __syncthreads();
+    if (empty) return;
+    const int lo = c0 * E - off, hi = (c0 + n * U) * E - off;
+    for (int k = tid; k < p.top_k; k += n) {
+      const int i = static_cast<int>(p.top_ids[r * p.top_k + k]);
+      if (i >= lo && i < hi && i >= 0 && i < V) {
+        const float v = grad2(pair(element(x + i))).x;
+        out[i] = static_cast<T>(v + p.g_top[r * p.top_k + k] + (i == t ? gl : 0.f));
+      }
+    }
+  }
+}
+
+template <typename T, bool kEnt, bool kTop>
+cudaError_t launch_fwd(const LogprobArgs& p, cudaStream_t st) {
+  const long long rows = p.batch * p.length;
+  const int chunks = (p.vocab * static_cast<long long>(sizeof(T)) + 15) / 16;
+  // fewer rows than SMs: a cluster a row, as long as a part keeps a thread of the smallest CTA
+  // busy
+  int parts = 1;
+  while (parts < kMaxCluster && rows * parts < kSms && chunks / (2 * parts) >= 128) parts *= 2;
+  const int per = chunks / parts;
+  const int threads = per >= 1024 ? 512 : (per >= 512 ? 256 : 128);
+  if (rows * parts > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  const size_t smem = kTop ? sizeof(TopShared) : 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * parts));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
+  return parts > 1 ? cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, kEnt, kTop, true>, p)
+                   : cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<T, kEnt, kTop, false>, p);
+}
+template <typename T>
+cudaError_t fwd_typed(const LogprobArgs& p, cudaStream_t st) {
+  // the entropy is also what a backward through it reads from the stats
+  if (p.entropy)
+    return p.top_k ? launch_fwd<T, true, true>(p, st) : launch_fwd<T, true, false>(p, st);
+  return p.top_k ? launch_fwd<T, false, true>(p, st) : launch_fwd<T, false, false>(p, st);
+}
+
+template <typename T, bool kEnt, bool kTop>
+cudaError_t launch_bwd(const LogprobArgs& p, cudaStream_t st) {
+  const long long rows = p.batch * p.length;
+  const int chunks = (p.vocab * static_cast<long long>(sizeof(T)) + 15) / 16 + 1;
+  const int threads = chunks >= 4 * 256 ? 256 : (chunks >= 4 * 128 ? 128 : 64);
+  const int parts = (chunks + threads * 4 - 1) / (threads * 4);
+  if (rows * parts > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  logprobs_bwd_kernel<T, kEnt, kTop>
+      <<<static_cast<unsigned>(rows * parts), threads, 0, st>>>(p, parts);
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t bwd_typed(const LogprobArgs& p, cudaStream_t st) {
+  if (p.g_entropy)
+    return p.g_top ? launch_bwd<T, true, true>(p, st) : launch_bwd<T, true, false>(p, st);
+  return p.g_top ? launch_bwd<T, false, true>(p, st) : launch_bwd<T, false, false>(p, st);
 }
 
 }  // namespace
 
 cudaError_t token_logprobs_fwd(const LogprobArgs& p, cudaStream_t st) {
-  const long long rows = p.batch * p.length;
-  const int grid = static_cast<int>(rows < 148 * 4 ? rows : 148 * 4);
-  logprobs_fwd_rows<<<grid, kLpThreads, 0, st>>>(p, rows);
-  return cudaGetLastError();
+  return p.f32 ? fwd_typed<float>(p, st) : fwd_typed<bf16>(p, st);
 }
-
 cudaError_t token_logprobs_bwd(const LogprobArgs& p, cudaStream_t st) {
-  const long long rows = p.batch * p.length;
-  const int grid = static_cast<int>(rows < 148 * 4 ? rows : 148 * 4);
-  logprobs_bwd_rows<<<grid, kLpThreads, 0, st>>>(p, rows);
-  return cudaGetLastError();
+  return p.f32 ? bwd_typed<float>(p, st) : bwd_typed<bf16>(p, st);
 }
 
 }  // namespace gmdn

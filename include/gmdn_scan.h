@@ -262,7 +262,8 @@ int gmdn_norm_bwd(const void* s, const float* rstd, const float* mean, const flo
  * no column), entropy of the row, and the top_k (at most 64) largest logits'
  * log probabilities and columns, in falling order, ties to the lowest column.
  * Any output may be NULL; top_k 0 writes no alternatives.  stats (rows, 4 fp32)
- * keeps what the backward needs, and may be NULL where there is none.  A row of
+ * keeps what the backward needs, and may be NULL where there is none (a backward
+ * through the entropy needs a forward that computed it).  A row of
  * nothing but -inf has logprob -inf, entropy 0 and a zero gradient; a row with
  * a NaN or +inf gives NaN (its alternatives are columns 0, 1, ...).  The
  * trainer's loss is its mean (train_ablation.py:197-246, 386-399). */
