@@ -64,13 +64,23 @@ __device__ __forceinline__ float2 pair(float a) { return make_float2(a, a); }
 struct Stat {
   float m, s, q;
 };
-__device__ __forceinline__ void join(Stat& a, const Stat& b) {
-  const float mn = fmaxf(a.m, b.m);
-  const float da = fmaxf(a.m - mn, kFar), db = fmaxf(b.m - mn, kFar);
-  const float fa = ex2(da * kLog2e), fb = ex2(db * kLog2e);
-  a.q = fa * fmaf(a.s, da, a.q) + fb * fmaf(b.s, db, b.q);
-  a.s = fa * a.s + fb * b.s;
-  a.m = mn;
+// A warp's threads joined: one maximum, every thread's sums brought to it, plain sums.  `kWidth`
+// lanes in all (a power of two); every lane gets the result.
+template <int kWidth>
+__device__ __forceinline__ Stat join_lanes(Stat a) {
+  float m = a.m;
+#pragma unroll
+  for (int o = kWidth / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  const float d = fmaxf(a.m - m, kFar), f = ex2(d * kLog2e);
+  a.q = f * fmaf(a.s, d, a.q);
+  a.s *= f;
+  a.m = m;
+#pragma unroll
+  for (int o = kWidth / 2; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(~0u, a.s, o);
+    a.q += __shfl_xor_sync(~0u, a.q, o);
+  }
+  return a;
 }
 
 // 16 bytes of a row
@@ -124,26 +134,30 @@ template <typename T>
 struct Row {
   static constexpr int E = Chunk<T>::E;
   const T* x;
-  int V, off, chunks;
+  int V, off, chunks, full0, full1;   // chunks full0 .. full1 - 1 lie wholly in the row
   __device__ __forceinline__ Row(const T* row, int vocab) : x(row), V(vocab) {
     off = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T));
     chunks = (off + V - 1) / E + 1;
+    full0 = off ? 1 : 0;
+    full1 = (off + V) / E;
+  }
+  __device__ __forceinline__ Chunk<T> load_full(int j) const {
+    const uint4 r = __ldg(reinterpret_cast<const uint4*>(x - off) + j);
+    Chunk<T> c;
+    c.w[0] = r.x;
+    c.w[1] = r.y;
+    c.w[2] = r.z;
+    c.w[3] = r.w;
+    return c;
   }
   __device__ __forceinline__ int first(int j) const { return j * E - off; }
   __device__ __forceinline__ Chunk<T> load(int j) const {
+    if (j >= full0 && j < full1) return load_full(j);
     const int i0 = first(j);
     Chunk<T> c;
-    if (i0 >= 0 && i0 <= V - E) {
-      const uint4 r = __ldg(reinterpret_cast<const uint4*>(x + i0));
-      c.w[0] = r.x;
-      c.w[1] = r.y;
-      c.w[2] = r.z;
-      c.w[3] = r.w;
-    } else {
 #pragma unroll
-      for (int k = 0; k < E; ++k)
-        c.set(k, i0 + k >= 0 && i0 + k < V ? element(x + i0 + k) : -INFINITY);
-    }
+    for (int k = 0; k < E; ++k)
+      c.set(k, i0 + k >= 0 && i0 + k < V ? element(x + i0 + k) : -INFINITY);
     return c;
   }
 };
@@ -162,32 +176,49 @@ __device__ __forceinline__ float key_value(unsigned long long k) {
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
-struct TopShared {
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+struct __align__(16) TopShared {
   unsigned long long above[kList], at[kList];
   unsigned long long best[kMaxTopK];
   float thread_max[kMaxThreads], group_max[kGroups];
   unsigned long long warp_best[kMaxThreads / 32];
   int warp_count[kMaxThreads / 32];
-  int n_above, n_at, have;
-  float bound;
+  int hot[kMaxThreads];   // threads whose maximum reaches the bound
+  int n_hot, n_above, n_at;
+  uint32_t bound;         // ordered()
 };
 
-// The place of key i among n keys, largest first.
+// The place of key k among n keys, largest first.  The keys' storage may be read up to the
+// next multiple of 8 (what lies there is not counted).
 __device__ __forceinline__ int place(const unsigned long long* keys, int n, unsigned long long k) {
   int r = 0;
-  for (int i = 0; i < n; ++i) r += keys[i] > k;
+  for (int i = 0; i < n; i += 8) {
+#pragma unroll
+    for (int u = 0; u < 8; u += 2) {
+      const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(keys + i + u);
+      r += (v.x > k && i + u < n) + (v.y > k && i + u + 1 < n);
+    }
+  }
   return r;
 }
 
-// The min(k, columns) largest columns of chunks [c0, c1) into sh.best, falling;
-// `mine`: the thread's largest value (at least -FLT_MAX) over chunks c0 + tid,
-// + blockDim, ....  No NaN among them.
+// The largest columns of chunks [c0, c1) into sh.best, falling: k of them, or all and then 0
+// (no column's key).  `mine`: the thread's largest value (at least -FLT_MAX) over chunks
+// c0 + tid, + blockDim, ....  In a row with NaN the result means nothing.
 template <typename T>
 __device__ void top_columns(TopShared& sh, const Row<T>& row, int c0, int c1, int k, float mine) {
   constexpr int E = Chunk<T>::E;
   const int tid = threadIdx.x, n = blockDim.x, lane = tid & 31, w = tid >> 5;
   sh.thread_max[tid] = mine;
-  if (tid == 0) sh.n_above = sh.n_at = 0;
+  if (tid < k) sh.best[tid] = 0;
+  if (tid == 0) {
+    sh.n_hot = sh.n_above = sh.n_at = 0;
+    sh.bound = 0;
+  }
   __syncthreads();
   if (tid < kGroups) {
     // groups of threads far apart: chunks that lie together fall into different groups
@@ -196,35 +227,49 @@ __device__ void top_columns(TopShared& sh, const Row<T>& row, int c0, int c1, in
     sh.group_max[tid] = g;
   }
   __syncthreads();
-  if (tid < kGroups) {
+  if (tid < kGroups) {   // the largest maximum that k of them reach
     const float g = sh.group_max[tid];
-    int r = 0;
+    int reach = 0;
 #pragma unroll 8
-    for (int t = 0; t < kGroups; ++t) {
-      const float o = sh.group_max[t];
-      r += o > g || (o == g && t < tid);
+    for (int t = 0; t < kGroups; t += 4) {
+      const float4 o = *reinterpret_cast<const float4*>(sh.group_max + t);
+      reach += (o.x >= g) + (o.y >= g) + (o.z >= g) + (o.w >= g);
     }
-    if (r == k - 1) sh.bound = g;
+    const uint32_t top = __reduce_max_sync(~0u, reach >= k ? ordered(g) : 0u);
+    if (lane == 0) atomicMax(&sh.bound, top);
   }
   __syncthreads();
-  const float bound = sh.bound;
+  const uint32_t ub = sh.bound;
+  const float bound = __uint_as_float((ub & 0x80000000u) ? (ub & 0x7fffffffu) : ~ub);
   const int lo = max(row.first(c0), 0), hi = min(row.first(c1), row.V);
   const int want = max(min(k, hi - lo), 0);
-  if (mine >= bound) {
-    for (int j = c0 + tid; j < c1; j += n) {
-      const Chunk<T> c = row.load(j);
-      if (!(c.largest() >= bound)) continue;
+  if (mine >= bound) sh.hot[atomicAdd(&sh.n_hot, 1)] = tid;
+  __syncthreads();
+  // the hot threads' chunks, 16 lanes a thread: read again, from L1 or L2
+  const int each = (c1 - c0 + n - 1) / n, n_hot = sh.n_hot;
+  auto keep = [&](const Chunk<T>& c, int j) {
+    if (!(c.largest() >= bound)) return;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float v = value(c, e);
-        const int i = row.first(j) + e;
-        if (v >= bound && i >= 0 && i < row.V) {
-          int* count = v > bound ? &sh.n_above : &sh.n_at;
-          unsigned long long* list = v > bound ? sh.above : sh.at;
-          const int slot = atomicAdd(count, 1);
-          if (slot < kList) list[slot] = key_of(v, i);
-        }
+    for (int e = 0; e < E; ++e) {
+      const float v = value(c, e);
+      const int col = row.first(j) + e;
+      if (v >= bound && col >= 0 && col < row.V) {
+        int* count = v > bound ? &sh.n_above : &sh.n_at;
+        unsigned long long* list = v > bound ? sh.above : sh.at;
+        const int slot = atomicAdd(count, 1);
+        if (slot < kList) list[slot] = key_of(v, col);
       }
+    }
+  };
+  for (int h = tid / 16; h < n_hot; h += n / 8) {
+    const int h2 = h + n / 16;
+    const int j0 = c0 + sh.hot[h], j1 = h2 < n_hot ? c0 + sh.hot[h2] : c1;
+    for (int i = (tid & 15) * n; i < each * n; i += 16 * n) {
+      Chunk<T> a, b;
+      if (j0 + i < c1) a = row.load(j0 + i);
+      if (j1 + i < c1) b = row.load(j1 + i);
+      if (j0 + i < c1) keep(a, j0 + i);
+      if (j1 + i < c1) keep(b, j1 + i);
     }
   }
   __syncthreads();
@@ -257,8 +302,6 @@ __device__ void top_columns(TopShared& sh, const Row<T>& row, int c0, int c1, in
       last = b;
       if (tid == 0) sh.best[r] = b;
     }
-    __syncthreads();
-    if (tid == 0) sh.have = want;
     __syncthreads();
     return;
   }
@@ -316,7 +359,6 @@ __device__ void top_columns(TopShared& sh, const Row<T>& row, int c0, int c1, in
     have = min(have + found, want);
     tie = -INFINITY;   // below the lowest finite value there is nothing else
   }
-  if (tid == 0) sh.have = want;
   __syncthreads();
 }
 
@@ -382,32 +424,79 @@ __global__ void __launch_bounds__(kMaxThreads) logprobs_fwd_kernel(LogprobArgs p
   float m = -FLT_MAX;
   float2 s = pair(0.f), q = pair(0.f);
   int j = c0 + tid;
-  for (; j + (kUnroll - 1) * n < c1; j += kUnroll * n) {
-    Chunk<T> c[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) c[u] = row.load(j + u * n);
-    absorb<T, kEnt, kUnroll>(c, m, s, q);
-  }
-  for (; j < c1; j += n) {
+  const int c1f = min(c1, row.full1);
+  if (j < row.full0) {   // a row's first chunk, if short
     const Chunk<T> c = row.load(j);
     absorb<T, kEnt, 1>(&c, m, s, q);
+    j += n;
+  }
+  for (; j + (kUnroll - 1) * n < c1f; j += kUnroll * n) {
+    Chunk<T> c[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) c[u] = row.load_full(j + u * n);
+    absorb<T, kEnt, kUnroll>(c, m, s, q);
+  }
+  for (; j < c1; j += kUnroll * n) {   // the rest, still kUnroll loads at a time
+    Chunk<T> c[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (j + u * n < c1) {
+        c[u] = row.load(j + u * n);
+      } else {
+#pragma unroll
+        for (int k = 0; k < Chunk<T>::E; ++k) c[u].set(k, -INFINITY);
+      }
+    }
+    absorb<T, kEnt, kUnroll>(c, m, s, q);
   }
   const float mine = m;
-  Stat a{m, s.x + s.y, q.x + q.y};
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    join(a, Stat{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o),
-                 __shfl_xor_sync(~0u, a.q, o)});
+  Stat a = join_lanes<32>(Stat{m, s.x + s.y, q.x + q.y});
   if (lane == 0) warp_stat[w] = a;
   __syncthreads();
-  a = warp_stat[0];
-  for (int k = 1; k < n / 32; ++k) join(a, warp_stat[k]);
+  if (kTop || w == 0) {   // the warps whose results are used
+    const int warps = n / 32;
+    a = lane % 16 < warps ? warp_stat[lane % 16] : Stat{-FLT_MAX, 0.f, 0.f};
+    a = join_lanes<16>(a);
+  }
+  TopShared& sh = *reinterpret_cast<TopShared*>(dyn);
+  if constexpr (kTop) top_columns(sh, row, c0, c1, p.top_k, mine);
   if constexpr (kCluster) {
+    // rank 0 takes the parts together: the stats, and the lists of alternatives
     auto cluster = cg::this_cluster();
     if (tid == 0) cta_stat = a;
     cluster.sync();
-    a = *cluster.map_shared_rank(&cta_stat, 0);
-    for (int k = 1; k < parts; ++k) join(a, *cluster.map_shared_rank(&cta_stat, k));
+    if (rank == 0) {
+      a = lane % 8 < parts ? *cluster.map_shared_rank(&cta_stat, lane % 8)
+                           : Stat{-FLT_MAX, 0.f, 0.f};
+      a = join_lanes<8>(a);
+      if constexpr (kTop) {
+        const int all = parts * p.top_k;
+        for (int i = tid; i < all; i += n)
+          sh.above[i] = cluster.map_shared_rank(&sh, i / p.top_k)->best[i % p.top_k];
+        __syncthreads();
+        // a column's place: its rank in every part's falling list, found by halving, all the
+        // lists a step at a time
+        for (int i = tid; i < all; i += n) {
+          const unsigned long long key = sh.above[i];
+          int ahead[kMaxCluster] = {};
+          for (int step = kMaxTopK; step > 0; step >>= 1) {
+            if (step > p.top_k) continue;
+#pragma unroll
+            for (int l = 0; l < kMaxCluster; ++l) {
+              const int to = ahead[l] + step;
+              if (l < parts && to <= p.top_k && sh.above[l * p.top_k + to - 1] > key) ahead[l] = to;
+            }
+          }
+          int at = 0;
+#pragma unroll
+          for (int l = 0; l < kMaxCluster; ++l) at += ahead[l];
+          if (key && at < p.top_k) sh.best[at] = key;
+        }
+        __syncthreads();
+      }
+    }
+    cluster.sync();   // the others' shared memory is read until here
+    if (rank != 0) return;
   }
   const bool empty = a.s == 0.f, bad = !(a.s >= 0.f) || a.m == INFINITY;
   const float ls = logf(a.s), nan = __int_as_float(0x7fffffff);
@@ -421,36 +510,11 @@ __global__ void __launch_bounds__(kMaxThreads) logprobs_fwd_kernel(LogprobArgs p
       p.logprobs[r] = t == p.ignore_index ? 0.f : (t >= 0 && t < p.vocab ? logprob(xt) : nan);
   }
   if constexpr (kTop) {
-    TopShared& sh = *reinterpret_cast<TopShared*>(dyn);
-    if (!bad) top_columns(sh, row, c0, c1, p.top_k, mine);
-    if constexpr (kCluster) {
-      // rank 0 takes the cluster's lists together
-      auto cluster = cg::this_cluster();
-      cluster.sync();
-      if (rank == 0 && !bad) {
-        int have = 0;
-        for (int k = 0; k < parts; ++k) {
-          const TopShared* other = cluster.map_shared_rank(&sh, k);
-          const int nk = other->have;
-          for (int i = tid; i < nk; i += n) sh.above[have + i] = other->best[i];
-          have += nk;
-        }
-        __syncthreads();
-        for (int i = tid; i < have; i += n) {
-          const int at = place(sh.above, have, sh.above[i]);
-          if (at < p.top_k) sh.best[at] = sh.above[i];
-        }
-        __syncthreads();
-      }
-      cluster.sync();   // the others' shared memory is read until here
-    }
-    if (rank == 0 && tid < p.top_k) {
+    if (tid < p.top_k) {
       const long long o = r * p.top_k + tid;
       p.top_ids[o] = bad ? tid : key_index(sh.best[tid]);
       p.top_logprobs[o] = bad ? nan : logprob(key_value(sh.best[tid]));
     }
-  } else if constexpr (kCluster) {
-    cg::this_cluster().sync();
   }
 }
 
@@ -607,7 +671,10 @@ cudaError_t launch_fwd(const LogprobArgs& p, cudaStream_t st) {
   int parts = 1;
   while (parts < kMaxCluster && rows * parts < kSms && chunks / (2 * parts) >= 128) parts *= 2;
   const int per = chunks / parts;
-  const int threads = per >= 1024 ? 512 : (per >= 512 ? 256 : 128);
+  // a CTA that has an SM to itself is bound by latency: as many threads as have a chunk; else
+  // enough chunks a thread to make up for what a CTA does once
+  const int big = rows * parts <= kSms ? 512 : 8192, mid = rows * parts <= kSms ? 256 : 1024;
+  const int threads = per >= big ? 512 : (per >= mid ? 256 : 128);
   if (rows * parts > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   const size_t smem = kTop ? sizeof(TopShared) : 0;
   cudaLaunchConfig_t cfg{};
