@@ -430,24 +430,30 @@ __global__ void __launch_bounds__(kMaxThreads) logprobs_fwd_kernel(LogprobArgs p
     absorb<T, kEnt, 1>(&c, m, s, q);
     j += n;
   }
-  for (; j + (kUnroll - 1) * n < c1f; j += kUnroll * n) {
-    Chunk<T> c[kUnroll];
+  // kUnroll chunks at a time, the next ones on their way while these are summed
+  auto fetch = [&](int at, Chunk<T>* c) {
+    if (at + (kUnroll - 1) * n < c1f) {
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) c[u] = row.load_full(j + u * n);
-    absorb<T, kEnt, kUnroll>(c, m, s, q);
-  }
-  for (; j < c1; j += kUnroll * n) {   // the rest, still kUnroll loads at a time
-    Chunk<T> c[kUnroll];
+      for (int u = 0; u < kUnroll; ++u) c[u] = row.load_full(at + u * n);
+      return;
+    }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      if (j + u * n < c1) {
-        c[u] = row.load(j + u * n);
+      if (at + u * n < c1) {
+        c[u] = row.load(at + u * n);
       } else {
 #pragma unroll
         for (int k = 0; k < Chunk<T>::E; ++k) c[u].set(k, -INFINITY);
       }
     }
-    absorb<T, kEnt, kUnroll>(c, m, s, q);
+  };
+  Chunk<T> now[kUnroll], next[kUnroll];
+  if (j < c1) fetch(j, now);
+  for (; j < c1; j += kUnroll * n) {
+    if (j + kUnroll * n < c1) fetch(j + kUnroll * n, next);
+    absorb<T, kEnt, kUnroll>(now, m, s, q);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) now[u] = next[u];
   }
   const float mine = m;
   Stat a = join_lanes<32>(Stat{m, s.x + s.y, q.x + q.y});
@@ -522,7 +528,7 @@ __global__ void __launch_bounds__(kMaxThreads) logprobs_fwd_kernel(LogprobArgs p
 // gradient
 // ---------------------------------------------------------------------------
 
-constexpr int kBwdThreads = 256;
+constexpr int kBwdThreads = 256;   // at most; at least kMaxTopK
 
 // Elements i0 .. i0 + E - 1 of a row that lies `shift` elements above a 16-byte
 // boundary there: the two aligned chunks that hold them, shifted together.
@@ -600,8 +606,19 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
     }
   }
   float wsum = gl;
-  if constexpr (kTop)
-    for (int k = 0; k < p.top_k; ++k) wsum += p.g_top[r * p.top_k + k];
+  // alternative `tid`, on its way while the row is worked on
+  int64_t top_i = -1;
+  float top_g = 0.f;
+  if constexpr (kTop) {
+    const int lane = tid & 31;
+    const float* gk = p.g_top + r * p.top_k;
+    if (tid < p.top_k) {
+      top_i = p.top_ids[r * p.top_k + tid];
+      top_g = gk[tid];
+    }
+    wsum += warp_sum((lane < p.top_k ? gk[lane] : 0.f) +
+                     (lane + 32 < p.top_k ? gk[lane + 32] : 0.f));
+  }
   const float A = kEnt ? -fmaf(gh, st.z, wsum) : -wsum, B = -gh;
   auto grad2 = [&](float2 v) {
     float2 lp = __fadd2_rn(__fadd2_rn(v, pair(-m)), pair(-ls));
@@ -649,16 +666,10 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
     }
   }
   if constexpr (kTop) {
+    const bool here = top_i >= max(c0 * E - off, 0) && top_i < min((c0 + n * U) * E - off, V);
+    const float v = here ? grad2(pair(element(x + top_i))).x + top_g + (top_i == t ? gl : 0.f) : 0.f;
     __syncthreads();
-    if (empty) return;
-    const int lo = c0 * E - off, hi = (c0 + n * U) * E - off;
-    for (int k = tid; k < p.top_k; k += n) {
-      const int i = static_cast<int>(p.top_ids[r * p.top_k + k]);
-      if (i >= lo && i < hi && i >= 0 && i < V) {
-        const float v = grad2(pair(element(x + i))).x;
-        out[i] = static_cast<T>(v + p.g_top[r * p.top_k + k] + (i == t ? gl : 0.f));
-      }
-    }
+    if (here && !empty) out[top_i] = static_cast<T>(v);
   }
 }
 
