@@ -38,20 +38,24 @@ __all__ = ["layer_norm", "rms_norm", "token_logprobs", "TokenLogprobs", "pack8",
            "Packed8", "act8_forward", "act8_backward", "Act8Saved", "mlp8"]
 
 MAX_TOP_K = 64
-_PLAIN = (Tensor, torch.nn.Parameter)
+_PLAIN = (Tensor, torch.nn.Parameter, type(None))
 
 
 def _eager(*tensors: Optional[Tensor]) -> bool:
     """Plain tensors, no tracing and no dispatch mode: nothing else has to see
     the call, so it may go to the library directly."""
-    return (not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0
-            and all(t is None or type(t) in _PLAIN for t in tensors))
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack():
+        return False
+    for t in tensors:
+        if type(t) not in _PLAIN:
+            return False
+    return True
 
 
 def _run(what: str, fn, device: torch.device, *args) -> None:
     """The library call on the device's current stream, with that device current."""
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -65,10 +69,14 @@ def _at(t: Optional[Tensor]) -> Optional[int]:
 
 
 def _same_device(name: str, first: Tensor, *others: Optional[Tensor]) -> None:
-    _require_cuda(name, first, *others)
+    """Every tensor on one CUDA device: a kernel would fault on another's memory."""
+    device = first.device
+    if device.type != "cuda":
+        _require_cuda(name, first)
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name}: tensors on {first.device} and {t.device}")
+        if t is not None and t.device != device:
+            _require_cuda(name, t)
+            raise ValueError(f"{name}: tensors on {device} and {t.device}")
 
 
 def _once(backward):
@@ -84,7 +92,11 @@ def _once(backward):
 
 
 def _needs_grad(*tensors: Optional[Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ---------------------------------------------------------------------------
@@ -93,18 +105,17 @@ def _needs_grad(*tensors: Optional[Tensor]) -> bool:
 
 def _norm_fwd_call(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor],
                    bias: Optional[Tensor], eps: float, center: bool,
-                   out_f32: bool) -> tuple[Tensor, Tensor, Tensor]:
+                   out_f32: bool) -> tuple[Tensor, Optional[Tensor], Tensor]:
     D = x.shape[-1]
     rows = x.numel() // D if D else 0
     y = torch.empty_like(x, dtype=torch.float32 if out_f32 else torch.bfloat16)
-    if residual is None:
-        h = x.new_empty(0)
-    else:
+    h = None
+    if residual is not None:
         h = torch.empty_like(residual if residual.dtype == torch.float32 else x)
     stats = torch.empty((2 if center else 1, rows), dtype=torch.float32, device=x.device)
     at = stats.data_ptr()
     _run("gmdn_norm_fwd", lib.gmdn_norm_fwd, x.device, x.data_ptr(), _at(residual), _at(weight),
-         _at(bias), y.data_ptr(), h.data_ptr(), at, at + 4 * rows if center else None, rows, D, eps,
+         _at(bias), y.data_ptr(), _at(h), at, at + 4 * rows if center else None, rows, D, eps,
          center, x.dtype == torch.float32,
          residual is not None and residual.dtype == torch.float32, out_f32)
     return y, h, stats
@@ -112,23 +123,20 @@ def _norm_fwd_call(x: Tensor, residual: Optional[Tensor], weight: Optional[Tenso
 
 def _norm_bwd_call(s: Tensor, stats: Tensor, weight: Optional[Tensor], dy: Tensor,
                    dh: Optional[Tensor], center: bool, want_bf16: bool, want_f32: bool,
-                   want_w: bool, want_b: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+                   want_w: bool, want_b: bool) -> tuple[Optional[Tensor], ...]:
     D = s.shape[-1]
     rows = s.numel() // D if D else 0
 
-    none = s.new_empty(0) if not (want_bf16 and want_f32 and want_w and want_b) else None
-    da = torch.empty_like(s, dtype=torch.bfloat16) if want_bf16 else none
-    db = torch.empty_like(s, dtype=torch.float32) if want_f32 else none
-    dweight = stats.new_empty(D) if want_w else none
-    dbias = stats.new_empty(D) if want_b else none
+    da = torch.empty_like(s, dtype=torch.bfloat16) if want_bf16 else None
+    db = torch.empty_like(s, dtype=torch.float32) if want_f32 else None
+    dweight = torch.empty(D, dtype=torch.float32, device=s.device) if want_w else None
+    dbias = torch.empty(D, dtype=torch.float32, device=s.device) if want_b else None
     nbytes = lib.gmdn_norm_bwd_workspace_bytes(rows, D) if want_w or want_b else 0
     ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device) if nbytes else None
     at = stats.data_ptr()
     _run("gmdn_norm_bwd", lib.gmdn_norm_bwd, s.device, s.data_ptr(), at,
          at + 4 * rows if center else None, _at(weight), dy.data_ptr(), _at(dh),
-         da.data_ptr() if want_bf16 else None, db.data_ptr() if want_f32 else None,
-         dweight.data_ptr() if want_w else None, dbias.data_ptr() if want_b else None, _at(ws),
-         nbytes, rows, D, center, s.dtype == torch.float32, dy.dtype == torch.float32,
+         _at(da), _at(db), _at(dweight), _at(dbias), _at(ws), nbytes, rows, D, center, s.dtype == torch.float32, dy.dtype == torch.float32,
          dh is not None and dh.dtype == torch.float32, False, True)
     return da, db, dweight, dbias
 
@@ -137,7 +145,8 @@ def _norm_bwd_call(s: Tensor, stats: Tensor, weight: Optional[Tensor], dy: Tenso
 def _norm_fwd(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor],
               bias: Optional[Tensor], eps: float, center: bool,
               out_f32: bool) -> tuple[Tensor, Tensor, Tensor]:
-    return _norm_fwd_call(x, residual, weight, bias, eps, center, out_f32)
+    y, h, stats = _norm_fwd_call(x, residual, weight, bias, eps, center, out_f32)
+    return y, x.new_empty(0) if h is None else h, stats
 
 
 @_norm_fwd.register_fake
@@ -154,10 +163,8 @@ def _norm_bwd(s: Tensor, stats: Tensor, weight: Optional[Tensor], dy: Tensor,
               dh: Optional[Tensor], center: bool, want_bf16: bool, want_f32: bool, want_w: bool,
               want_b: bool) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     got = _norm_bwd_call(s, stats, weight, dy, dh, center, want_bf16, want_f32, want_w, want_b)
-    wanted = (want_bf16, want_f32, want_w, want_b)
     types = (torch.bfloat16, torch.float32, torch.float32, torch.float32)
-    # an op's outputs are tensors of their own
-    return tuple(g if w else s.new_empty(0, dtype=t) for g, w, t in zip(got, wanted, types))
+    return tuple(s.new_empty(0, dtype=t) if g is None else g for g, t in zip(got, types))
 
 
 @_norm_bwd.register_fake
@@ -188,7 +195,7 @@ def _norm_backward(ctx, dy, dh, _dstats):
     elif dh is not None:
         dh = _aligned(dh)
     need = ctx.needs_input_grad
-    wanted = {t for t, n in zip(ctx.types, need) if n}
+    wanted = [t for t, n in zip(ctx.types, need) if n]
     call = _norm_bwd_call if _eager(s, dy, dh) else torch.ops.gmdn.norm_bwd
     da, db, dweight, dbias = call(s, stats, weight, dy, dh, ctx.center, torch.bfloat16 in wanted,
                                   torch.float32 in wanted, need[2], need[3])
@@ -216,7 +223,7 @@ def _norm(name: str, center: bool, x: Tensor, weight: Optional[Tensor], bias: Op
         raise ValueError(f"{name}: x must have a last axis to normalise")
     D = x.shape[-1]
     for what, t in (("weight", weight), ("bias", bias)):
-        if t is not None and tuple(t.shape) != (D,):
+        if t is not None and t.shape != (D,):
             raise ValueError(f"{name}: {what} must be ({D},), got {tuple(t.shape)}")
     if residual is not None and residual.shape != x.shape:
         raise ValueError(f"{name}: residual {tuple(residual.shape)} != x {tuple(x.shape)}")
@@ -302,23 +309,23 @@ def _rows_of(logits: Tensor):
 
 
 def _logprobs_fwd_call(logits: Tensor, targets: Optional[Tensor], entropy: bool, top_k: int,
-                       ignore_index: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+                       ignore_index: int) -> tuple[Optional[Tensor], ...]:
     shape, V = logits.shape[:-1], logits.shape[-1]
     if (rows := _rows_of(logits)) is None:
         logits = logits.contiguous()
         rows = _rows_of(logits)
 
     stats = torch.empty((*shape, 4), dtype=torch.float32, device=logits.device)
-    lp = stats.new_empty(shape if targets is not None else 0)
-    ent = stats.new_empty(shape if entropy else 0)
-    tops = stats.new_empty((*shape, top_k) if top_k else 0)
-    ids = torch.empty((*shape, top_k) if top_k else 0, dtype=torch.int64, device=logits.device)
+    lp = stats.new_empty(shape) if targets is not None else None
+    ent = stats.new_empty(shape) if entropy else None
+    tops = ids = None
+    if top_k:
+        tops = stats.new_empty((*shape, top_k))
+        ids = torch.empty((*shape, top_k), dtype=torch.int64, device=logits.device)
     b, t, sb, st = rows
     _run("gmdn_token_logprobs_fwd", lib.gmdn_token_logprobs_fwd, logits.device, logits.data_ptr(),
-         _at(targets), lp.data_ptr() if targets is not None else None,
-         ent.data_ptr() if entropy else None, tops.data_ptr() if top_k else None,
-         ids.data_ptr() if top_k else None, stats.data_ptr(), b, t, sb, st, V, top_k, ignore_index,
-         logits.dtype == torch.float32)
+         _at(targets), _at(lp), _at(ent), _at(tops), _at(ids), stats.data_ptr(), b, t, sb, st, V,
+         top_k, ignore_index, logits.dtype == torch.float32)
     return lp, ent, tops, ids, stats
 
 
@@ -340,7 +347,9 @@ def _logprobs_bwd_call(logits: Tensor, targets: Optional[Tensor], ids: Optional[
 @torch.library.custom_op("gmdn::token_logprobs_fwd", mutates_args=())
 def _logprobs_fwd(logits: Tensor, targets: Optional[Tensor], entropy: bool, top_k: int,
                   ignore_index: int) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
-    return _logprobs_fwd_call(logits, targets, entropy, top_k, ignore_index)
+    *got, stats = _logprobs_fwd_call(logits, targets, entropy, top_k, ignore_index)
+    types = (torch.float32, torch.float32, torch.float32, torch.int64)
+    return (*(logits.new_empty(0, dtype=t) if g is None else g for g, t in zip(got, types)), stats)
 
 
 @_logprobs_fwd.register_fake
@@ -370,7 +379,8 @@ def _(logits, targets, ids, stats, g_lp, g_ent, g_top, ignore_index):
 def _logprobs_setup(ctx, inputs, output):
     logits, targets, entropy, top_k, ignore_index = inputs
     _, _, _, ids, stats = output
-    ctx.mark_non_differentiable(ids)
+    if ids is not None:
+        ctx.mark_non_differentiable(ids)
     ctx.save_for_backward(logits, targets, ids if top_k else None, stats)
     ctx.ignore_index, ctx.entropy = ignore_index, entropy
     ctx.set_materialize_grads(False)
