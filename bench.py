@@ -613,7 +613,7 @@ def run_train(args) -> None:
     inner = {0: "delta", 1: "muon", 2: "adam"}[CONFIGS[args.config]["rule"]]
     torch.manual_seed(0)
     model = tr.LanguageModel(vocab, d, layers, heads, inner, chunk=64, ns_steps=3,
-                             mlp=args.mlp).to(device)
+                             mlp=args.mlp, fused=args.fused, act8=args.act8).to(device)
     net = model
     if dist is not None:
         net = torch.nn.parallel.DistributedDataParallel(model, device_ids=[local],
@@ -648,17 +648,20 @@ def run_train(args) -> None:
         dist.barrier()
     ms = pkg.sharding.max_over_ranks(ms, device)
     tokens = world * mb * T * args.steps
+    peak_gb = torch.cuda.max_memory_allocated(device) / 1e9
     line = {
         "metric": "config-4 training tokens/s (12-layer GMDN LM, d768, H12, vocab 32000, seq 2048)",
         "value": tokens / (ms / 1e3), "unit": "tokens/s", "n_gpus": world, "steps": args.steps,
         "warmup": max(args.warmup, 3), "ms_per_step": ms / args.steps, "higher_is_better": True,
         "scaling": "weak", "vs_baseline": None, "dtype": "bf16", "data": "synthetic",
         "config": {"workload": "config4_train", "inner": inner, "mlp": args.mlp,
+                   "fused": args.fused, "act8": args.act8,
                    "micro_batch_per_gpu": mb,
                    "global_batch": world * mb, "seq_len": T, "layers": layers, "d_model": d,
                    "heads": heads, "vocab": vocab,
                    "parallelism": f"dp{world}" + (" (DDP, NCCL all-reduce)" if world > 1 else ""),
                    "params_M": sum(p.numel() for p in model.parameters()) / 1e6},
+        "peak_memory_GB": peak_gb,
         "loss_first_last": [float(losses[0]), float(losses[-1])],
         "lr_schedule": "train_ablation.py's: linear warm-up over 500 steps, these are steps "
                        f"0-{max(args.warmup, 3) + args.steps - 1}",
@@ -787,6 +790,11 @@ def main():
     ap.add_argument("--mlp", default="gelu", choices=["gelu", "swiglu"],
                     help="train workload: the reference trainer's GELU MLP, or the SwiGLU MLP "
                          "that the config-4 benchmark description names")
+    ap.add_argument("--fused", action="store_true",
+                    help="train workload: norms with their residual adds and the loss on the "
+                         "library's kernels")
+    ap.add_argument("--act8", action="store_true",
+                    help="train workload: the MLPs keep their activations in 8 bits")
     ap.add_argument("--scaling", default="strong", choices=["weak", "strong"],
                     help="strong (default): the one global batch the metric names split into "
                          "(b, h) shards over the ranks; weak: a full batch per rank.  At N > 1 "
