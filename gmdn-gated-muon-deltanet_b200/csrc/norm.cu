@@ -101,9 +101,22 @@ __device__ __forceinline__ void load_param(const float* p, int i, float* v) {
   }
 }
 
-// Sums of two values over a row's threads; every thread gets both.  A CTA's
-// row takes one barrier: `red` alternates between two buffers of 64 floats, so
-// a warp that is ahead writes the other one.
+// Sums of one value or two over a row's threads; every thread gets them.  A
+// CTA's row takes one barrier: `red` alternates between two buffers of 64
+// floats, so a warp that is ahead writes the other one.
+template <bool kCta>
+__device__ __forceinline__ void row_sum(float& a, float*& red) {
+  a = warp_sum(a);
+  if constexpr (kCta) {
+    const int lane = threadIdx.x & 31, n = blockDim.x >> 5;
+    if (lane == 0) red[threadIdx.x >> 5] = a;
+    __syncthreads();
+    a = (lane & 15) < n ? red[lane & 15] : 0.f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) a += __shfl_xor_sync(~0u, a, o);
+    red = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(red) ^ 256);
+  }
+}
 template <bool kCta>
 __device__ __forceinline__ void row_sums(float& a, float& b, float*& red) {
   a = warp_sum(a);
@@ -118,6 +131,22 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float*& red) {
     a = warp_sum(lane < n ? red[lane] : 0.f);
     b = warp_sum(lane < n ? red[32 + lane] : 0.f);
     red = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(red) ^ 256);
+  }
+}
+
+// v rounded to bf16, in place, pairs at a time
+template <int VEC>
+__device__ __forceinline__ void round_bf16(float* v) {
+  if constexpr (VEC == 1) {
+    v[0] = __bfloat162float(__float2bfloat16_rn(v[0]));
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[k], v[k + 1]);
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(&h);
+      v[k] = __uint_as_float(w << 16);
+      v[k + 1] = __uint_as_float(w & 0xffff0000u);
+    }
   }
 }
 
@@ -155,8 +184,7 @@ norm_fwd_regs(NormFwdArgs p) {
   fetch(r);
   for (; r < p.rows; r += step) {
     const size_t base = static_cast<size_t>(r) * D;
-    float s[NV][VEC];
-    float sum = 0.f, unused = 0.f;
+    float s[NV][VEC], sum = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int g = v * tpr + tid;
@@ -165,20 +193,19 @@ norm_fwd_regs(NormFwdArgs p) {
         s[v][k] = 0.f;
         if (g < groups) {
           s[v][k] = rx[v].get(k);
-          if constexpr (kRes) {
-            s[v][k] += rr[v].get(k);
-            if constexpr (!kHf32) s[v][k] = __bfloat162float(__float2bfloat16_rn(s[v][k]));
-          }
+          if constexpr (kRes) s[v][k] += rr[v].get(k);
         }
-        sum += s[v][k];
       }
+      if constexpr (kRes && !kHf32) round_bf16<VEC>(s[v]);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sum += s[v][k];
       if constexpr (kRes)
         if (g < groups) store_group<VEC>(p.h, base + g * VEC, s[v], kHf32);
     }
     fetch(r + step);
     float mean = 0.f;
     if (p.center) {
-      row_sums<kCta>(sum, unused, red);
+      row_sum<kCta>(sum, red);
       mean = sum * inv;
     }
     float d1 = 0.f, d2 = 0.f;
@@ -427,8 +454,8 @@ __global__ void __launch_bounds__(kMaxCta, NV == 8 ? 2 : 1) norm_fwd_ring(NormFw
       }
       sum += s[v];
     }
-    // one barrier here whatever `center` is: it also frees the stage
-    row_sums<true>(sum, d2, red);
+    // here whatever `center` is: the barrier also frees the stage
+    row_sum<true>(sum, red);
     float mean = p.center ? sum * inv : 0.f;
     float d1 = 0.f;
 #pragma unroll
@@ -688,8 +715,8 @@ __global__ void __launch_bounds__(kColThreads) norm_bwd_cols(NormBwdArgs p, int 
 
 // dw, db from the partials, in a fixed order (bit-reproducible): 32 columns a
 // CTA, each warp every 32nd partial, blockIdx.y 0: dw, 1: db.
-constexpr int kJoinWarps = 32;
-__global__ void __launch_bounds__(kJoinWarps * 32) norm_bwd_join(const float* partial, float* dw,
+constexpr int kJoinWarps = 32, kJoinFly = 5;
+__global__ void __launch_bounds__(kJoinWarps * 32, 1024 / (kJoinWarps * 16)) norm_bwd_join(const float* partial, float* dw,
                                                                  float* db, int D, int parts) {
   __shared__ float red[kJoinWarps][33];
   float* out = blockIdx.y == 0 ? dw : db;
@@ -698,15 +725,26 @@ __global__ void __launch_bounds__(kJoinWarps * 32) norm_bwd_join(const float* pa
   const int col = blockIdx.x * 32 + lane;
   float a = 0.f;
   if (col < D) {
-#pragma unroll 4
-    for (int k = w; k < parts; k += kJoinWarps)
-      a += partial[(static_cast<size_t>(k) * 2 + blockIdx.y) * D + col];
+    const float* src = partial + static_cast<size_t>(blockIdx.y) * D + col;
+    for (int k0 = w; k0 < parts; k0 += kJoinWarps * kJoinFly) {
+      float v[kJoinFly];   // all in flight: the kernel is nothing but their latency
+#pragma unroll
+      for (int u = 0; u < kJoinFly; ++u) {
+        const int k = k0 + u * kJoinWarps;
+        v[u] = k < parts ? __ldcg(src + static_cast<size_t>(k) * 2 * D) : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < kJoinFly; ++u) a += v[u];
+    }
   }
   red[w][lane] = a;
   __syncthreads();
-  const float t = warp_sum(red[lane][w]);   // warp w: column w of the 32
-  const int c = blockIdx.x * 32 + w;
-  if (lane == 0 && c < D) out[c] = t;
+  if (w == 0 && col < D) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < kJoinWarps; ++k) t += red[k][lane];
+    out[col] = t;
+  }
 }
 
 int row_grid(long long rows) {
