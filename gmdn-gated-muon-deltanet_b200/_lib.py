@@ -11,6 +11,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libgmdn_b200.so")
+TORCH_LIB_PATH = os.path.join(_HERE, "libgmdn_torch.so")
 
 GMDN_PREC_IEEE = 0
 GMDN_PREC_FAST = 1
@@ -107,6 +108,16 @@ lib.gmdn_act8_fwd.restype = _i
 lib.gmdn_act8_fwd.argtypes = [_p] * 7 + [_q, _i, _p]
 lib.gmdn_act8_bwd.restype = _i
 lib.gmdn_act8_bwd.argtypes = [_p] * 8 + [_q, _i, _p]
+
+
+def load_torch_ops() -> None:
+    """Register the operators of ``libgmdn_torch.so`` (torch.ops.gmdn.*)."""
+    import torch
+    if not os.path.exists(TORCH_LIB_PATH):
+        raise ImportError(
+            f"{TORCH_LIB_PATH} is missing: build it with "
+            f"`python {os.path.join(_HERE, 'build.py')}`")
+    torch.ops.load_library(TORCH_LIB_PATH)
 
 
 def check(rc: int, what: str) -> None:

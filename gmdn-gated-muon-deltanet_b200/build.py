@@ -6,6 +6,8 @@ Every ``csrc/*.cu`` file is compiled by nvcc for ``sm_100a`` only
 (``-gencode arch=compute_100a,code=sm_100a``) into ``_build/`` and linked into
 ``libgmdn_b200.so`` next to this file.  The library exposes the C ABI of
 ``include/gmdn_scan.h`` and nothing else; it does not depend on torch.
+``csrc/torch_ops.cpp`` (torch operators over that ABI) becomes
+``libgmdn_torch.so``, which links it and the installed torch.
 A file is recompiled only when it or any header it may include is newer than
 its object, so repeated calls are cheap.
 """
@@ -15,6 +17,7 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -25,6 +28,8 @@ ROOT = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 BUILD = os.path.join(PKG_DIR, "_build")
 LIB = os.path.join(PKG_DIR, "libgmdn_b200.so")
+TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_LIB = os.path.join(PKG_DIR, "libgmdn_torch.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-Xptxas", "-warn-spills"]
@@ -58,6 +63,33 @@ def _compile(src: str, obj: str, extra: list[str]) -> tuple[str, str]:
     return src, res.stderr
 
 
+def _torch_dir() -> str:
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("torch not found: libgmdn_torch.so is built against it")
+    return spec.submodule_search_locations[0]
+
+
+def build_torch(force: bool = False) -> str:
+    """libgmdn_torch.so: plain C++ (no device code), against the installed torch."""
+    header = max(os.path.getmtime(h) for h in glob.glob(os.path.join(ROOT, "include", "*.h")))
+    if not force and not _stale(TORCH_SRC, TORCH_LIB, header):
+        return TORCH_LIB
+    t = _torch_dir()
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-D_GLIBCXX_USE_CXX11_ABI=1", "-I", os.path.join(t, "include"),
+           "-I", os.path.join(t, "include", "torch", "csrc", "api", "include"),
+           "-I", os.path.join(cuda, "include"), TORCH_SRC, "-o", TORCH_LIB + ".tmp",
+           "-L", os.path.join(t, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-L", PKG_DIR,
+           "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {os.path.basename(TORCH_SRC)}:\n{res.stdout}\n{res.stderr}")
+    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    return TORCH_LIB
+
+
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
           extra: list[str] | None = None) -> str:
     os.makedirs(BUILD, exist_ok=True)
@@ -80,6 +112,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(LIB + ".tmp", LIB)
+    build_torch(force)
     return LIB
 
 

@@ -851,7 +851,7 @@ def test_offsets_past_32_bits():
     want = 5.0 - math.log(V - 2 + math.exp(5.0) + math.exp(6.0))
     assert abs(got.logprobs[-1].item() - want) < 1e-5
     assert got.top_ids[-1].tolist() == [V - 1, 777] and got.top_ids[0].tolist() == [0, 1]
-    g = pkg.step_ops._logprobs_bwd_call(
+    g = torch.ops.gmdn.token_logprobs_bwd(
         z, torch.full((rows,), 777, device="cuda"), None,
         torch.tensor([[0.0, math.log(V), math.log(V), 0.0]], device="cuda").expand(rows, 4)
         .contiguous(), torch.ones(rows, device="cuda"), None, None, -100)
