@@ -23,13 +23,6 @@ __device__ __forceinline__ void cp_async_cg16(void* smem, const void* gmem) {
                "l"(gmem)
                : "memory");
 }
-// the same, of the first `bytes` (0..16) from gmem; the rest is zeros and not read
-__device__ __forceinline__ void cp_async_cg16(void* smem, const void* gmem, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                   static_cast<uint32_t>(__cvta_generic_to_shared(smem))),
-               "l"(gmem), "r"(bytes)
-               : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
 }

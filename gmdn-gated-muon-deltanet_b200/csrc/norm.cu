@@ -19,37 +19,49 @@
 #include <type_traits>
 
 #include "common.cuh"
-#include "cp_async.cuh"
 #include "step_ops.h"
 
 namespace gmdn {
 namespace {
 
 // ---------------------------------------------------------------------------
-// Rows in registers.  A row is held by one warp (short rows, four a CTA, no
-// barrier) or by one CTA; each thread has NV groups of VEC
-// consecutive elements of it, group v * threads + thread.  VEC is 8 where the
-// width is a multiple of 8, so that every row starts 16-byte aligned and a
-// group is one or two 16-byte accesses; short rows of other widths go element
-// by element (VEC 1), longer ones through shared memory (below).
-// A thread walks rows grid apart: the next row's loads are issued as soon as
-// the current one's registers are converted, before its reductions, so memory
-// is busy while the row is summed.
+// Rows in registers.  A row is held by part of a warp, a warp (short rows, no
+// barrier) or a CTA; each thread has NV groups of 8 consecutive elements of it,
+// group v * threads + thread, each one or two 16-byte accesses a tensor.  A
+// thread walks rows grid apart: the next row's loads are issued as soon as the
+// current one's registers are converted, before its reductions, so memory is
+// busy while the row is summed.
+//
+// Where the width is no multiple of 8, rows start at any place of the groups
+// of 8 elements that the memory falls into.  The grid's step is then a multiple
+// of 8 rows, so a thread sees one such place, `off` elements into its first
+// group, in all its rows: it loads the groups of the row whole (the first and
+// the last hold elements of the rows beside, which it masks out), keeps the same
+// columns throughout, and finds the weights in a copy in shared memory that is
+// shifted by `off`.
 // ---------------------------------------------------------------------------
 
 constexpr int kSms = 148;
-constexpr int kRowWarps = 4;     // warp rows of a CTA
+constexpr int kRowThreads = 128; // CTA of warp rows
 constexpr int kMaxCta = 512;     // threads of a CTA row: 128 registers each
-constexpr int kMaxResident = 4;  // CTAs an SM, at most: each writes a partial of dw and db
 using bf16 = __nv_bfloat16;
 
-template <typename T, int VEC>
-struct Raw {   // VEC 8
+template <typename T>
+struct Raw {   // 8 consecutive elements as loaded
   uint4 r[sizeof(T) / 2];
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
     for (int k = 0; k < static_cast<int>(sizeof(T)) / 2; ++k)
       r[k] = __ldcs(reinterpret_cast<const uint4*>(p) + k);
+  }
+  // the first n of them (the tensor ends there)
+  __device__ __forceinline__ void load_some(const T* p, int n) {
+    T v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = k < n ? p[k] : static_cast<T>(0.f);
+#pragma unroll
+    for (int k = 0; k < static_cast<int>(sizeof(T)) / 2; ++k)
+      r[k] = reinterpret_cast<const uint4*>(v)[k];
   }
   __device__ __forceinline__ float get(int k) const {
     if constexpr (sizeof(T) == 2) {
@@ -61,25 +73,14 @@ struct Raw {   // VEC 8
     }
   }
 };
-template <typename T>
-struct Raw<T, 1> {
-  T r;
-  __device__ __forceinline__ void load(const T* p) { r = __ldcs(p); }
-  __device__ __forceinline__ float get(int) const { return static_cast<float>(r); }
-};
-template <>
-struct Raw<bf16, 1> {
-  uint16_t r;
-  __device__ __forceinline__ void load(const bf16* p) {
-    r = __ldcs(reinterpret_cast<const unsigned short*>(p));
-  }
-  __device__ __forceinline__ float get(int) const { return bf16_to_f32(r); }
-};
 
-template <int VEC>
-__device__ __forceinline__ void store_group(void* base, size_t i, const float* v, bool f32) {
-  if constexpr (VEC == 1) {
-    store_act(base, i, v[0], f32);
+// 8 elements at i, those of `mask` (0xff: all, one or two 16-byte stores)
+__device__ __forceinline__ void store_group(void* base, size_t i, const float* v, bool f32,
+                                            uint32_t mask) {
+  if (mask != 0xffu) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (mask >> k & 1) store_act(base, i + k, v[k], f32);
   } else if (f32) {
     float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + i);
     p[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -91,37 +92,32 @@ __device__ __forceinline__ void store_group(void* base, size_t i, const float* v
     *reinterpret_cast<uint4*>(static_cast<bf16*>(base) + i) = *reinterpret_cast<uint4*>(h);
   }
 }
-template <int VEC>
-__device__ __forceinline__ void load_param(const float* p, int i, float* v) {
-  if constexpr (VEC == 1) {
-    v[0] = __ldg(p + i);
-  } else {
-    *reinterpret_cast<float4*>(v) = __ldg(reinterpret_cast<const float4*>(p + i));
-    *reinterpret_cast<float4*>(v + 4) = __ldg(reinterpret_cast<const float4*>(p + i) + 1);
-  }
-}
 
-// Sums of one value or two over a row's threads; every thread gets them.  A
-// CTA's row takes one barrier: `red` alternates between two buffers of 64
-// floats, so a warp that is ahead writes the other one.
-template <bool kCta>
+// Sums over a row's threads; every thread gets them.  LPR lanes of a warp a row,
+// or (0) a CTA: one barrier, `red` alternating between two buffers of 64
+// floats, so that a warp that is ahead writes the other one.
+template <int LPR>
+__device__ __forceinline__ float lane_sum(float v) {
+#pragma unroll
+  for (int o = (LPR ? LPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+template <int LPR>
 __device__ __forceinline__ void row_sum(float& a, float*& red) {
-  a = warp_sum(a);
-  if constexpr (kCta) {
+  a = lane_sum<LPR>(a);
+  if constexpr (LPR == 0) {
     const int lane = threadIdx.x & 31, n = blockDim.x >> 5;
     if (lane == 0) red[threadIdx.x >> 5] = a;
     __syncthreads();
-    a = (lane & 15) < n ? red[lane & 15] : 0.f;
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a += __shfl_xor_sync(~0u, a, o);
+    a = warp_sum(lane < n ? red[lane] : 0.f);
     red = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(red) ^ 256);
   }
 }
-template <bool kCta>
+template <int LPR>
 __device__ __forceinline__ void row_sums(float& a, float& b, float*& red) {
-  a = warp_sum(a);
-  b = warp_sum(b);
-  if constexpr (kCta) {
+  a = lane_sum<LPR>(a);
+  b = lane_sum<LPR>(b);
+  if constexpr (LPR == 0) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, n = blockDim.x >> 5;
     if (lane == 0) {
       red[w] = a;
@@ -134,92 +130,168 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float*& red) {
   }
 }
 
-// v rounded to bf16, in place, pairs at a time
-template <int VEC>
+// 8 values rounded to bf16, in place, pairs at a time
 __device__ __forceinline__ void round_bf16(float* v) {
-  if constexpr (VEC == 1) {
-    v[0] = __bfloat162float(__float2bfloat16_rn(v[0]));
-  } else {
 #pragma unroll
-    for (int k = 0; k < VEC; k += 2) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(v[k], v[k + 1]);
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(&h);
-      v[k] = __uint_as_float(w << 16);
-      v[k + 1] = __uint_as_float(w & 0xffff0000u);
-    }
+  for (int k = 0; k < 8; k += 2) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[k], v[k + 1]);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&h);
+    v[k] = __uint_as_float(w << 16);
+    v[k + 1] = __uint_as_float(w & 0xffff0000u);
   }
 }
 
 struct None {};
 
-template <typename TX, typename TR, int VEC, int NV, bool kCta>
-__global__ void __launch_bounds__(kCta ? kMaxCta : kRowWarps * 32, kCta && NV == 2 ? 2 : 1)
+// Where a thread's part of its rows lies.
+template <int NV, int LPR, bool kOdd>
+struct Place {
+  static constexpr int kSlots = LPR ? kRowThreads / LPR : 1;   // rows a CTA has at a time
+  int tid, tpr, slot, lead, off, width;
+  long long row, step;        // the thread's first row; `lead` more than its warp's first
+  uint32_t mask[kOdd ? NV : 1];   // kOdd: the row's elements of each group
+  __device__ __forceinline__ Place(int D) : width(D) {
+    tid = LPR ? threadIdx.x % (LPR ? LPR : 1) : threadIdx.x;
+    tpr = LPR ? LPR : blockDim.x;
+    slot = LPR ? threadIdx.x / (LPR ? LPR : 1) : 0;
+    lead = LPR ? slot % (32 / (LPR ? LPR : 32)) : 0;
+    row = static_cast<long long>(blockIdx.x) * kSlots + slot;
+    step = static_cast<long long>(gridDim.x) * kSlots;
+    off = 0;
+    if constexpr (kOdd) {
+      off = static_cast<int>((row % 8 * (D % 8)) % 8);
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int c = group(v) * 8 - off;   // the group's first column
+        mask[v] = 0;
+        if (c < D)
+          mask[v] = (c < 0 ? 0xffu << -c & 0xffu : 0xffu) &
+                    (D - c < 8 ? 0xffu >> (8 - (D - c)) : 0xffu);
+      }
+    }
+  }
+  // whether the row reaches into group v, lies all over it, and its elements there
+  __device__ __forceinline__ bool has(int v) const {
+    return kOdd ? mask[kOdd ? v : 0] != 0 : group(v) * 8 < width;
+  }
+  __device__ __forceinline__ bool whole(int v) const { return !kOdd || mask[kOdd ? v : 0] == 0xffu; }
+  __device__ __forceinline__ uint32_t bits(int v) const { return kOdd ? mask[kOdd ? v : 0] : 0xffu; }
+  __device__ __forceinline__ int group(int v) const { return v * tpr + tid; }
+  // the row's first group as an element of the tensor
+  __device__ __forceinline__ size_t base(long long r, int D) const {
+    return static_cast<size_t>(r) * D - off;
+  }
+  template <typename T>
+  __device__ __forceinline__ void load(Raw<T>& raw, const T* p, size_t i, size_t total) const {
+    if (!kOdd || i + 8 <= total)
+      raw.load(p + i);
+    else
+      raw.load_some(p + i, static_cast<int>(total - i));
+  }
+  // a (width) parameter's shared copy for this thread's slot: column c at off + c, 0 around
+  static __host__ __device__ int copy_floats(int D) { return (D + 14) / 8 * 8; }
+  __device__ __forceinline__ void copy(float* dst, const float* src, int D) const {
+    for (int i = tid; i < copy_floats(D); i += tpr) {
+      const int c = i - off;
+      dst[i] = c >= 0 && c < D ? src[c] : 0.f;
+    }
+  }
+  // 8 values of a parameter for group v
+  __device__ __forceinline__ void param(const float* global, const float* shared, int v,
+                                        float* q) const {
+    const float4* p = reinterpret_cast<const float4*>((kOdd ? shared : global) + group(v) * 8);
+    *reinterpret_cast<float4*>(q) = kOdd ? p[0] : __ldg(p);
+    *reinterpret_cast<float4*>(q + 4) = kOdd ? p[1] : __ldg(p + 1);
+  }
+};
+
+template <typename TX, typename TR, int NV, int LPR, bool kOdd>
+__global__ void __launch_bounds__(LPR ? kRowThreads : kMaxCta,
+                                  LPR == 0 && NV == 2 && !kOdd && sizeof(TX) + sizeof(TR) < 8 ? 2 : 1)
 norm_fwd_regs(NormFwdArgs p) {
   constexpr bool kRes = !std::is_same<TR, None>::value;
   using TL = typename std::conditional<kRes, TR, TX>::type;   // the residual's loads
   constexpr bool kHf32 = std::is_same<TX, float>::value || std::is_same<TR, float>::value;
   __shared__ __align__(512) float buf[128];
+  extern __shared__ __align__(16) float params[];   // kOdd: weight, bias, a copy a slot
   float* red = buf;
-  const int tid = kCta ? threadIdx.x : threadIdx.x & 31, tpr = kCta ? blockDim.x : 32;
-  const int D = p.width, groups = D / VEC;
+  const int D = p.width;
   const float inv = 1.f / static_cast<float>(D);
-  const long long step = static_cast<long long>(gridDim.x) * (kCta ? 1 : kRowWarps);
-  long long r = kCta ? blockIdx.x
-                     : static_cast<long long>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
+  const size_t total = static_cast<size_t>(p.rows) * D;
+  const Place<NV, LPR, kOdd> at(D);
+  float *sw = nullptr, *sb = nullptr;
+  if constexpr (kOdd) {
+    const int n = at.copy_floats(D);
+    sw = params + at.slot * n;
+    sb = sw + (p.weight ? at.kSlots * n : 0);
+    if (p.weight) at.copy(sw, p.weight, D);
+    if (p.bias) at.copy(sb, p.bias, D);
+    __syncthreads();
+  }
   const TX* x = static_cast<const TX*>(p.x);
   const TL* res = static_cast<const TL*>(p.res);
-  Raw<TX, VEC> rx[NV];
-  Raw<TL, VEC> rr[NV];
+  Raw<TX> rx[NV];
+  Raw<TL> rr[NV];
   auto fetch = [&](long long row) {
     if (row >= p.rows) return;
+    const size_t base = at.base(row, D);
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int g = v * tpr + tid;
-      if (g < groups) {
-        rx[v].load(x + row * D + g * VEC);
-        if constexpr (kRes) rr[v].load(res + row * D + g * VEC);
+    for (int v = 0; v < NV; ++v)
+      if (at.has(v)) {
+        at.load(rx[v], x, base + at.group(v) * 8, total);
+        if constexpr (kRes) at.load(rr[v], res, base + at.group(v) * 8, total);
       }
-    }
   };
-  fetch(r);
-  for (; r < p.rows; r += step) {
-    const size_t base = static_cast<size_t>(r) * D;
-    float s[NV][VEC], sum = 0.f;
+  fetch(at.row);
+  // a warp's rows go together: its lanes meet in the sums whether they have a row or not
+  for (long long r = at.row; r - at.lead < p.rows; r += at.step) {
+    const bool live = LPR == 0 || LPR == 32 || r < p.rows;
+    const size_t base = at.base(r, D);
+    float s[NV][8], sum = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int g = v * tpr + tid;
+      const bool in = at.has(v) && live;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
+      for (int k = 0; k < 8; ++k) {
         s[v][k] = 0.f;
-        if (g < groups) {
+        if (in && (!kOdd || at.bits(v) >> k & 1)) {
           s[v][k] = rx[v].get(k);
           if constexpr (kRes) s[v][k] += rr[v].get(k);
         }
       }
-      if constexpr (kRes && !kHf32) round_bf16<VEC>(s[v]);
+      if constexpr (kRes && !kHf32) round_bf16(s[v]);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) sum += s[v][k];
+      for (int k = 0; k < 8; ++k) sum += s[v][k];
       if constexpr (kRes)
-        if (g < groups) store_group<VEC>(p.h, base + g * VEC, s[v], kHf32);
+        if (in) store_group(p.h, base + at.group(v) * 8, s[v], kHf32, at.bits(v));
     }
-    fetch(r + step);
+    fetch(r + at.step);
     float mean = 0.f;
     if (p.center) {
-      row_sum<kCta>(sum, red);
+      row_sum<LPR>(sum, red);
       mean = sum * inv;
     }
     float d1 = 0.f, d2 = 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
-      if (v * tpr + tid < groups) {
+      if (at.has(v)) {
+        if (!at.whole(v)) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const float d = s[v][k] - mean;
-          d1 += d;
-          d2 = fmaf(d, d, d2);
+          for (int k = 0; k < 8; ++k) {
+            const float d = at.bits(v) >> k & 1 ? s[v][k] - mean : 0.f;
+            d1 += d;
+            d2 = fmaf(d, d, d2);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float d = s[v][k] - mean;
+            d1 += d;
+            d2 = fmaf(d, d, d2);
+          }
         }
       }
-    row_sums<kCta>(d1, d2, red);
+    row_sums<LPR>(d1, d2, red);
     d2 *= inv;
     if (p.center) {   // what the rounding of the mean left, taken out of both
       d1 *= inv;
@@ -227,94 +299,98 @@ norm_fwd_regs(NormFwdArgs p) {
       d2 = fmaxf(d2 - d1 * d1, 0.f);
     }
     const float rstd = rsqrtf(d2 + p.eps);
-    if (tid == 0) {
+    if (at.tid == 0 && live) {
       p.rstd[r] = rstd;
       if (p.center) p.mean[r] = mean;
     }
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int g = v * tpr + tid;
-      if (g < groups) {
-        float q[VEC];
+    for (int v = 0; v < NV; ++v)
+      if (at.has(v) && live) {
+        float q[8];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) s[v][k] = (s[v][k] - mean) * rstd;
+        for (int k = 0; k < 8; ++k) s[v][k] = (s[v][k] - mean) * rstd;
         if (p.weight) {
-          load_param<VEC>(p.weight, g * VEC, q);
+          at.param(p.weight, sw, v, q);
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) s[v][k] *= q[k];
+          for (int k = 0; k < 8; ++k) s[v][k] *= q[k];
         }
         if (p.bias) {
-          load_param<VEC>(p.bias, g * VEC, q);
+          at.param(p.bias, sb, v, q);
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) s[v][k] += q[k];
+          for (int k = 0; k < 8; ++k) s[v][k] += q[k];
         }
-        store_group<VEC>(p.y, base + g * VEC, s[v], p.y_f32);
+        store_group(p.y, base + at.group(v) * 8, s[v], p.y_f32, at.bits(v));
       }
-    }
   }
 }
 
 // TS: the type of s and dh.  dw and db are summed over a thread's rows in
 // registers; a CTA's sums are one partial (norm_bwd_join adds the partials).
-template <typename TS, typename TG, int VEC, int NV, bool kCta, bool kDb>
-__global__ void __launch_bounds__(kCta ? kMaxCta : kRowWarps * 32)
+// kMaxThreads: an odd width's masks do not fit the 128 registers of 512 threads; up to 256
+// they have 255.
+template <typename TS, typename TG, int NV, int LPR, bool kOdd, bool kDb, int kMaxThreads>
+__global__ void __launch_bounds__(LPR ? kRowThreads : kMaxThreads)
 norm_bwd_regs(NormBwdArgs p) {
   __shared__ __align__(512) float buf[128];
-  extern __shared__ float cols[];   // warp rows: kRowWarps x D
+  extern __shared__ __align__(16) float dyn[];   // kOdd: weight copies; then a warp row's sums
   float* red = buf;
-  const int tid = kCta ? threadIdx.x : threadIdx.x & 31, tpr = kCta ? blockDim.x : 32;
-  const int D = p.width, groups = D / VEC;
+  const int D = p.width;
   const float inv = 1.f / static_cast<float>(D);
-  const long long step = static_cast<long long>(gridDim.x) * (kCta ? 1 : kRowWarps);
-  long long r = kCta ? blockIdx.x
-                     : static_cast<long long>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
+  const size_t total = static_cast<size_t>(p.rows) * D;
+  const Place<NV, LPR, kOdd> at(D);
+  float* sw = nullptr;
+  if constexpr (kOdd) {
+    sw = dyn + at.slot * at.copy_floats(D);
+    if (p.weight) at.copy(sw, p.weight, D);
+    __syncthreads();
+  }
   const TS *sp = static_cast<const TS*>(p.s), *dhp = static_cast<const TS*>(p.dh);
   const TG* gp = static_cast<const TG*>(p.dy);
-  Raw<TS, VEC> rs[NV], rh[NV];
-  Raw<TG, VEC> rg[NV];
+  Raw<TS> rs[NV], rh[NV];
+  Raw<TG> rg[NV];
   float rstd_next = 0.f, mean_next = 0.f;
   auto fetch = [&](long long row) {
     if (row >= p.rows) return;
     rstd_next = p.rstd[row];
     mean_next = p.center ? p.mean[row] : 0.f;
+    const size_t base = at.base(row, D);
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int g = v * tpr + tid;
-      if (g < groups) {
-        rs[v].load(sp + row * D + g * VEC);
-        rg[v].load(gp + row * D + g * VEC);
+    for (int v = 0; v < NV; ++v)
+      if (at.has(v)) {
+        at.load(rs[v], sp, base + at.group(v) * 8, total);
+        at.load(rg[v], gp, base + at.group(v) * 8, total);
       }
-    }
   };
-  float dw[NV][VEC], db[kDb ? NV : 1][VEC];
+  float dw[NV][8], db[kDb ? NV : 1][8];
 #pragma unroll
   for (int v = 0; v < NV; ++v)
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
+    for (int k = 0; k < 8; ++k) {
       dw[v][k] = 0.f;
       if constexpr (kDb) db[v][k] = 0.f;
     }
-  fetch(r);
-  for (; r < p.rows; r += step) {
-    const size_t base = static_cast<size_t>(r) * D;
+  fetch(at.row);
+  for (long long r = at.row; r - at.lead < p.rows; r += at.step) {
+    const bool live = LPR == 0 || LPR == 32 || r < p.rows;
+    const size_t base = at.base(r, D);
     const float rstd = rstd_next, mean = mean_next;
-    float xh[NV][VEC], g[NV][VEC];
+    float xh[NV][8], g[NV][8];
     float a = 0.f, b = 0.f;
-    if (dhp) {   // needed last: in flight over the reduction, not a row ahead
+    if (dhp && live) {   // needed last: in flight over the reduction, not a row ahead
 #pragma unroll
       for (int v = 0; v < NV; ++v)
-        if (v * tpr + tid < groups) rh[v].load(dhp + base + (v * tpr + tid) * VEC);
+        if (at.has(v)) at.load(rh[v], dhp, base + at.group(v) * 8, total);
     }
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = v * tpr + tid;
-      if (i < groups) {
-        float w[VEC];
-        if (p.weight) load_param<VEC>(p.weight, i * VEC, w);
+    for (int v = 0; v < NV; ++v)
+      if (at.has(v) && live) {
+        float w[8];
+        if (p.weight) at.param(p.weight, sw, v, w);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
+        for (int k = 0; k < 8; ++k) {
           xh[v][k] = (rs[v].get(k) - mean) * rstd;
           g[v][k] = rg[v].get(k);
+          if (kOdd && !(at.bits(v) >> k & 1)) xh[v][k] = g[v][k] = 0.f;
           dw[v][k] = fmaf(g[v][k], xh[v][k], dw[v][k]);
           if constexpr (kDb) db[v][k] += g[v][k];
           if (p.weight) g[v][k] *= w[k];
@@ -322,285 +398,96 @@ norm_bwd_regs(NormBwdArgs p) {
           b = fmaf(g[v][k], xh[v][k], b);
         }
       }
-    }
-    fetch(r + step);
-    row_sums<kCta>(a, b, red);
+    fetch(r + at.step);
+    row_sums<LPR>(a, b, red);
     a = p.center ? a * inv : 0.f;
     b *= inv;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = v * tpr + tid;
-      if (i < groups) {
+    for (int v = 0; v < NV; ++v)
+      if (at.has(v) && live) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k)
+        for (int k = 0; k < 8; ++k)
           g[v][k] = fmaf(fmaf(xh[v][k], -b, g[v][k] - a), rstd, dhp ? rh[v].get(k) : 0.f);
-        if (p.ds_a) store_group<VEC>(p.ds_a, base + i * VEC, g[v], p.a_f32);
-        if (p.ds_b) store_group<VEC>(p.ds_b, base + i * VEC, g[v], p.b_f32);
+        if (p.ds_a) store_group(p.ds_a, base + at.group(v) * 8, g[v], p.a_f32, at.bits(v));
+        if (p.ds_b) store_group(p.ds_b, base + at.group(v) * 8, g[v], p.b_f32, at.bits(v));
       }
-    }
   }
   if (!p.dw && !p.db) return;
   float* out = p.partial + static_cast<size_t>(blockIdx.x) * 2 * D;
 #pragma unroll
   for (int which = 0; which < (kDb ? 2 : 1); ++which) {
-    float* dst = kCta ? out + which * D : cols + (threadIdx.x >> 5) * D;
-    if (!kCta && which == 1) __syncthreads();   // cols is read below
+    // CTA rows write the partial; warp rows their slot of `dyn` (over the weight copies)
+    float* dst = LPR ? dyn + at.slot * D : out + which * D;
+    if constexpr (LPR != 0) __syncthreads();
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = v * tpr + tid;
-      if (i < groups) {
+    for (int v = 0; v < NV; ++v)
+      if (at.has(v)) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
+        for (int k = 0; k < 8; ++k) {
           float t = dw[v][k];
           if constexpr (kDb) t = which ? db[v][k] : t;
-          dst[i * VEC + k] = t;
+          if (at.bits(v) >> k & 1) dst[at.group(v) * 8 - at.off + k] = t;
         }
       }
-    }
-    if constexpr (!kCta) {
+    if constexpr (LPR != 0) {
       __syncthreads();
-      for (int c = threadIdx.x; c < D; c += kRowWarps * 32) {
+      for (int c = threadIdx.x; c < D; c += kRowThreads) {
         float t = 0.f;
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) t += cols[w * D + c];
+        for (int w = 0; w < at.kSlots; ++w) t += dyn[w * D + c];
         out[which * D + c] = t;
       }
     }
   }
 }
 
-// ---------------------------------------------------------------------------
-// Rows whose width is no multiple of 8 start at any alignment.  One CTA a row:
-// the row's 16-byte chunks, whole ones from the boundary below its start to the
-// one above its end, come into a ring in shared memory by cp.async kStages - 1
-// rows ahead (the last chunk of the tensor is cut to its end), and a thread
-// reads its elements, v * threads + thread, from there.  With element-wise loads
-// from global memory instead there are too few bytes in flight.  Every read of a
-// stage is before the row's first sum, whose barrier lets the next issue
-// overwrite it.
-// ---------------------------------------------------------------------------
-
-constexpr int kStages = 4;
-
-__host__ __device__ inline int stage_bytes(int D, int es) { return (D * es + 46) / 16 * 16; }
-
-template <typename T>
-__device__ __forceinline__ void issue_row(char* dst, const void* base, size_t e0, int D,
-                                          size_t total) {
-  constexpr int E = 16 / static_cast<int>(sizeof(T));
-  const size_t a0 = e0 / E * E;
-  const int chunks = (static_cast<int>(e0 - a0) + D + E - 1) / E;
-  const T* src = static_cast<const T*>(base) + a0;
-  const size_t left = total - a0;
-  for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
-    const size_t rest = left - static_cast<size_t>(c) * E;
-    cp_async_cg16(dst + 16 * c, src + static_cast<size_t>(c) * E,
-                  rest < E ? static_cast<uint32_t>(rest) * sizeof(T) : 16u);
-  }
-}
-// the row's element i
-template <typename T>
-__device__ __forceinline__ float stage_at(const char* src, size_t e0, int i) {
-  constexpr int E = 16 / static_cast<int>(sizeof(T));
-  const int at = static_cast<int>(e0 % E) + i;
-  if constexpr (sizeof(T) == 2)
-    return bf16_to_f32(reinterpret_cast<const uint16_t*>(src)[at]);
-  else
-    return reinterpret_cast<const float*>(src)[at];
-}
-
-template <typename TX, typename TR, int NV>
-__global__ void __launch_bounds__(kMaxCta, NV == 8 ? 2 : 1) norm_fwd_ring(NormFwdArgs p) {
-  constexpr bool kRes = !std::is_same<TR, None>::value;
-  using TL = typename std::conditional<kRes, TR, TX>::type;
-  constexpr bool kHf32 = std::is_same<TX, float>::value || std::is_same<TR, float>::value;
-  __shared__ __align__(512) float buf[128];
-  extern __shared__ __align__(16) char ring[];
-  float* red = buf;
-  const int tid = threadIdx.x, tpr = blockDim.x, D = p.width;
-  const float inv = 1.f / static_cast<float>(D);
-  const size_t total = static_cast<size_t>(p.rows) * D;
-  const int bx = stage_bytes(D, sizeof(TX)), stage = bx + (kRes ? stage_bytes(D, sizeof(TL)) : 0);
-  auto issue = [&](long long row, int k) {
-    if (row < p.rows) {
-      const size_t e0 = static_cast<size_t>(row) * D;
-      issue_row<TX>(ring + k * stage, p.x, e0, D, total);
-      if constexpr (kRes) issue_row<TL>(ring + k * stage + bx, p.res, e0, D, total);
-    }
-    cp_async_commit();
-  };
-  for (int k = 0; k < kStages - 1; ++k)
-    issue(blockIdx.x + static_cast<long long>(k) * gridDim.x, k);
-  int at = 0;
-  for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    issue(r + static_cast<long long>(kStages - 1) * gridDim.x, (at + kStages - 1) % kStages);
-    cp_async_wait<kStages - 1>();
-    __syncthreads();
-    const size_t base = static_cast<size_t>(r) * D;
-    const char* src = ring + at * stage;
-    at = (at + 1) % kStages;
-    float s[NV], sum = 0.f, d2 = 0.f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = v * tpr + tid;
-      s[v] = 0.f;
-      if (i < D) {
-        s[v] = stage_at<TX>(src, base, i);
-        if constexpr (kRes) {
-          s[v] += stage_at<TL>(src + bx, base, i);
-          if constexpr (!kHf32) s[v] = __bfloat162float(__float2bfloat16_rn(s[v]));
-          store_act(p.h, base + i, s[v], kHf32);
-        }
-      }
-      sum += s[v];
-    }
-    // here whatever `center` is: the barrier also frees the stage
-    row_sum<true>(sum, red);
-    float mean = p.center ? sum * inv : 0.f;
-    float d1 = 0.f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-      if (v * tpr + tid < D) {
-        const float d = s[v] - mean;
-        d1 += d;
-        d2 = fmaf(d, d, d2);
-      }
-    row_sums<true>(d1, d2, red);
-    d2 *= inv;
-    if (p.center) {
-      d1 *= inv;
-      mean += d1;
-      d2 = fmaxf(d2 - d1 * d1, 0.f);
-    }
-    const float rstd = rsqrtf(d2 + p.eps);
-    if (tid == 0) {
-      p.rstd[r] = rstd;
-      if (p.center) p.mean[r] = mean;
-    }
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = v * tpr + tid;
-      if (i < D) {
-        float y = (s[v] - mean) * rstd;
-        if (p.weight) y *= __ldg(p.weight + i);
-        if (p.bias) y += __ldg(p.bias + i);
-        store_act(p.y, base + i, y, p.y_f32);
-      }
-    }
-  }
-  cp_async_wait<0>();
-}
-
-template <typename TS, typename TG, int NV>
-__global__ void __launch_bounds__(kMaxCta, 1) norm_bwd_ring(NormBwdArgs p) {
-  __shared__ __align__(512) float buf[128];
-  extern __shared__ __align__(16) char ring[];
-  float* red = buf;
-  const int tid = threadIdx.x, tpr = blockDim.x, D = p.width;
-  const float inv = 1.f / static_cast<float>(D);
-  const size_t total = static_cast<size_t>(p.rows) * D;
-  const int bs = stage_bytes(D, sizeof(TS)), bg = stage_bytes(D, sizeof(TG));
-  const int stage = bs + bg + (p.dh ? bs : 0);
-  auto issue = [&](long long row, int k) {
-    if (row < p.rows) {
-      const size_t e0 = static_cast<size_t>(row) * D;
-      issue_row<TS>(ring + k * stage, p.s, e0, D, total);
-      issue_row<TG>(ring + k * stage + bs, p.dy, e0, D, total);
-      if (p.dh) issue_row<TS>(ring + k * stage + bs + bg, p.dh, e0, D, total);
-    }
-    cp_async_commit();
-  };
-  for (int k = 0; k < kStages - 1; ++k)
-    issue(blockIdx.x + static_cast<long long>(k) * gridDim.x, k);
-  float dw[NV], db[NV];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) dw[v] = db[v] = 0.f;
-  int at = 0;
-  for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    issue(r + static_cast<long long>(kStages - 1) * gridDim.x, (at + kStages - 1) % kStages);
-    const float rstd = p.rstd[r], mean = p.center ? p.mean[r] : 0.f;
-    cp_async_wait<kStages - 1>();
-    __syncthreads();
-    const size_t base = static_cast<size_t>(r) * D;
-    const char* src = ring + at * stage;
-    at = (at + 1) % kStages;
-    float xh[NV], g[NV], dh[NV], a = 0.f, b = 0.f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = v * tpr + tid;
-      if (i < D) {
-        xh[v] = (stage_at<TS>(src, base, i) - mean) * rstd;
-        g[v] = stage_at<TG>(src + bs, base, i);
-        dh[v] = p.dh ? stage_at<TS>(src + bs + bg, base, i) : 0.f;
-        dw[v] = fmaf(g[v], xh[v], dw[v]);
-        db[v] += g[v];
-        if (p.weight) g[v] *= __ldg(p.weight + i);
-        a += g[v];
-        b = fmaf(g[v], xh[v], b);
-      }
-    }
-    row_sums<true>(a, b, red);
-    a = p.center ? a * inv : 0.f;
-    b *= inv;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = v * tpr + tid;
-      if (i < D) {
-        const float d = fmaf(fmaf(xh[v], -b, g[v] - a), rstd, dh[v]);
-        if (p.ds_a) store_act(p.ds_a, base + i, d, p.a_f32);
-        if (p.ds_b) store_act(p.ds_b, base + i, d, p.b_f32);
-      }
-    }
-  }
-  cp_async_wait<0>();
-  if (!p.dw && !p.db) return;
-  float* out = p.partial + static_cast<size_t>(blockIdx.x) * 2 * D;
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int i = v * tpr + tid;
-    if (i < D) {
-      out[i] = dw[v];
-      out[D + i] = db[v];
-    }
-  }
-}
-
-// How a width is held.  VEC 8: warp rows up to 768 elements (three groups a
-// lane are as many as the backward's five arrays of them leave registers for),
-// CTA rows with two groups a thread up to 8192, in the forward with four up to
-// 16384.  VEC 1: warp rows up to 256, then the ring with 8 elements a thread up
-// to 4096, 16 up to 8192 (as far as its stages fit).  Wider rows are read again
-// for each pass (threads 0).
+// How a width is held: by the most groups of 8 a row can touch.  Rows of up to
+// 96 groups by 8, 16 or 32 lanes (three groups a lane are as many as the
+// backward's five arrays of them leave registers for); CTA rows with two groups
+// a thread up to 1024, in the forward with four up to 2048.  Wider rows are read
+// again for each pass (lanes -1).
 struct Shape {
-  int vec, nv, threads;   // threads 32: warp rows
+  int nv, lanes, threads;   // lanes 0: CTA rows
+  bool odd;
 };
 Shape shape_of(int D, bool fwd) {
-  auto up = [](int n, int per) { return (n + per * 32 - 1) / (per * 32) * 32; };
-  if (D % 8 == 0) {
-    if (D <= 768) return {8, (D + 255) / 256, 32};
-    if (D <= 16 * kMaxCta) return {8, 2, up(D, 16)};
-    if (fwd && D <= 32 * kMaxCta) return {8, 4, up(D, 32)};
-  } else if (D <= 256) {
-    return {1, 8, 32};
-  } else if (D <= 8 * kMaxCta) {
-    return {1, 8, up(D, 8)};
-  } else if (D <= 16 * kMaxCta) {
-    return {1, 16, up(D, 16)};
-  }
-  return {0, 0, 0};
+  const bool odd = D % 8 != 0;
+  const int groups = odd ? (D + 14) / 8 : D / 8;
+  auto up = [&](int per) { return (groups + per * 32 - 1) / (per * 32) * 32; };
+  if (groups <= 8) return {1, 8, kRowThreads, odd};
+  if (groups <= 16) return {1, 16, kRowThreads, odd};
+  if (groups <= 96) return {(groups + 31) / 32, 32, kRowThreads, odd};
+  if (groups <= 2 * kMaxCta) return {2, 0, up(2), odd};
+  if (fwd && groups <= 4 * kMaxCta) return {4, 0, up(4), odd};
+  return {0, -1, 0, odd};
 }
-constexpr size_t kMaxRing = 220 * 1024;   // shared memory the ring's stages may take
+int slots_of(Shape sh) { return sh.lanes > 0 ? kRowThreads / sh.lanes : 1; }
 
-// One wave of CTAs, each walking rows a grid apart.
+// One wave of CTAs, each walking rows a grid apart; for odd widths the step is a
+// multiple of 8 rows.
 template <typename K>
-int wave(K kernel, long long rows, int threads, size_t smem) {
-  const long long want = threads == 32 ? (rows + kRowWarps - 1) / kRowWarps : rows;
-  if (want <= kSms) return static_cast<int>(want);
-  int n = 1;
-  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads == 32 ? kRowWarps * 32 : threads,
-                                                smem);
-  const long long cap = static_cast<long long>(kSms) * (n < 1 ? 1 : n);
-  return static_cast<int>(want < cap ? want : cap);
+int wave(K kernel, long long rows, Shape sh, size_t smem) {
+  const int slots = slots_of(sh);
+  const long long want = (rows + slots - 1) / slots;
+  long long grid = want;
+  if (want > kSms) {
+    int n = 1;
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, sh.threads, smem);
+    const long long cap = static_cast<long long>(kSms) * (n < 1 ? 1 : n);
+    if (cap < grid) grid = cap;
+  }
+  if (sh.odd && grid < want && slots % 8) {
+    const int per = 8 / slots > 0 ? 8 / slots : 1;
+    grid = grid / per * per;
+  }
+  return static_cast<int>(grid);
+}
+
+template <typename K>
+cudaError_t allow(K kernel, size_t smem) {
+  return smem <= 48 * 1024 ? cudaSuccess
+                           : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                  static_cast<int>(smem));
 }
 
 // ---------------------------------------------------------------------------
@@ -609,7 +496,6 @@ int wave(K kernel, long long rows, int threads, size_t smem) {
 
 constexpr int kColThreads = 256;
 constexpr int kColRows = 8;      // warps of a column block, each on every 8th row
-constexpr int kMaxPartials = 296;
 
 // One CTA a row, any width: the row is read again for each pass (from L1 / L2).
 __global__ void __launch_bounds__(kThreads) norm_fwd_rows(NormFwdArgs p) {
@@ -751,89 +637,76 @@ int row_grid(long long rows) {
   return static_cast<int>(rows < kSms * 8 ? rows : kSms * 8);
 }
 
-template <typename TX, typename TR, int VEC, int NV, bool kCta>
-void fwd_go(const NormFwdArgs& p, Shape sh, cudaStream_t st) {
-  auto k = norm_fwd_regs<TX, TR, VEC, NV, kCta>;
-  k<<<wave(k, p.rows, sh.threads, 0), kCta ? sh.threads : kRowWarps * 32, 0, st>>>(p);
-}
-// A ring kernel of this much shared memory, one wave; the stages of up to 8192
-// elements of three fp32 tensors do not fit four times, so such rows are refused
-// here and read again for each pass.
-template <typename K>
-cudaError_t allow(K kernel, size_t smem) {
-  return smem <= 48 * 1024 ? cudaSuccess
-                           : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                  static_cast<int>(smem));
-}
-size_t ring_fwd(const NormFwdArgs& p) {
-  return kStages * (stage_bytes(p.width, p.x_f32 ? 4 : 2) +
-                    (p.res ? stage_bytes(p.width, p.res_f32 ? 4 : 2) : 0));
-}
-size_t ring_bwd(const NormBwdArgs& p) {
-  return kStages * (stage_bytes(p.width, p.s_f32 ? 4 : 2) * (p.dh ? 2 : 1) +
-                    stage_bytes(p.width, p.dy_f32 ? 4 : 2));
-}
-template <typename TX, typename TR, int NV>
-cudaError_t fwd_ring(const NormFwdArgs& p, Shape sh, cudaStream_t st) {
-  auto k = norm_fwd_ring<TX, TR, NV>;
-  const size_t smem = ring_fwd(p);
+template <typename TX, typename TR, int NV, int LPR, bool kOdd>
+cudaError_t fwd_go(const NormFwdArgs& p, Shape sh, cudaStream_t st) {
+  auto k = norm_fwd_regs<TX, TR, NV, LPR, kOdd>;
+  const size_t copy = Place<NV, LPR, kOdd>::copy_floats(p.width) * sizeof(float) * slots_of(sh);
+  const size_t smem = kOdd ? copy * ((p.weight ? 1 : 0) + (p.bias ? 1 : 0)) : 0;
   cudaError_t e = allow(k, smem);
   if (e != cudaSuccess) return e;
-  k<<<wave(k, p.rows, sh.threads, smem), sh.threads, smem, st>>>(p);
+  k<<<wave(k, p.rows, sh, smem), sh.threads, smem, st>>>(p);
   return cudaGetLastError();
+}
+template <typename TX, typename TR, bool kOdd>
+cudaError_t fwd_shaped(const NormFwdArgs& p, Shape sh, cudaStream_t st) {
+  if (sh.lanes == 8) return fwd_go<TX, TR, 1, 8, kOdd>(p, sh, st);
+  if (sh.lanes == 16) return fwd_go<TX, TR, 1, 16, kOdd>(p, sh, st);
+  if (sh.lanes == 32) {
+    if (sh.nv == 1) return fwd_go<TX, TR, 1, 32, kOdd>(p, sh, st);
+    if (sh.nv == 2) return fwd_go<TX, TR, 2, 32, kOdd>(p, sh, st);
+    return fwd_go<TX, TR, 3, 32, kOdd>(p, sh, st);
+  }
+  if (sh.nv == 2) return fwd_go<TX, TR, 2, 0, kOdd>(p, sh, st);
+  return fwd_go<TX, TR, 4, 0, kOdd>(p, sh, st);
 }
 template <typename TX, typename TR>
 cudaError_t fwd_typed(const NormFwdArgs& p, Shape sh, cudaStream_t st) {
-  if (sh.threads == 32) {
-    if (sh.vec == 1) fwd_go<TX, TR, 1, 8, false>(p, sh, st);
-    else if (sh.nv == 1) fwd_go<TX, TR, 8, 1, false>(p, sh, st);
-    else if (sh.nv == 2) fwd_go<TX, TR, 8, 2, false>(p, sh, st);
-    else fwd_go<TX, TR, 8, 3, false>(p, sh, st);
-  } else {
-    if (sh.vec == 1) return sh.nv == 8 ? fwd_ring<TX, TR, 8>(p, sh, st) : fwd_ring<TX, TR, 16>(p, sh, st);
-    if (sh.nv == 2) fwd_go<TX, TR, 8, 2, true>(p, sh, st);
-    else fwd_go<TX, TR, 8, 4, true>(p, sh, st);
-  }
-  return cudaGetLastError();
+  return sh.odd ? fwd_shaped<TX, TR, true>(p, sh, st) : fwd_shaped<TX, TR, false>(p, sh, st);
 }
 
-template <typename TS, typename TG, bool kDb, int VEC, int NV, bool kCta>
-int bwd_go(const NormBwdArgs& p, Shape sh, int most, cudaStream_t st) {
-  auto k = norm_bwd_regs<TS, TG, VEC, NV, kCta, kDb>;
-  const size_t smem = !kCta && (p.dw || p.db) ? sizeof(float) * kRowWarps * p.width : 0;
-  int grid = wave(k, p.rows, sh.threads, smem);
-  if (grid > most) grid = most;
-  k<<<grid, kCta ? sh.threads : kRowWarps * 32, smem, st>>>(p);
-  return grid;
-}
-template <typename TS, typename TG, int NV>
-int bwd_ring(const NormBwdArgs& p, Shape sh, int most, cudaStream_t st) {
-  auto k = norm_bwd_ring<TS, TG, NV>;
-  const size_t smem = ring_bwd(p);
-  if (allow(k, smem) != cudaSuccess) return 0;
-  int grid = wave(k, p.rows, sh.threads, smem);
-  if (grid > most) grid = most;
+// Launches the rows' kernel with at most `most` CTAs; *parts: how many there are.
+template <typename TS, typename TG, bool kDb, bool kOdd, int NV, int LPR, int kMaxThreads = kMaxCta>
+cudaError_t bwd_go(const NormBwdArgs& p, Shape sh, int most, int* parts, cudaStream_t st) {
+  auto k = norm_bwd_regs<TS, TG, NV, LPR, kOdd, kDb, kMaxThreads>;
+  const int slots = slots_of(sh);
+  const size_t copies = kOdd && p.weight ? Place<NV, LPR, kOdd>::copy_floats(p.width) * slots : 0;
+  const size_t sums = LPR && (p.dw || p.db) ? static_cast<size_t>(p.width) * slots : 0;
+  const size_t smem = sizeof(float) * (copies > sums ? copies : sums);
+  cudaError_t e = allow(k, smem);
+  if (e != cudaSuccess) return e;
+  int grid = wave(k, p.rows, sh, smem);
+  if (grid > most) grid = most;   // a multiple of 8
+  *parts = grid;
   k<<<grid, sh.threads, smem, st>>>(p);
-  return grid;
+  return cudaGetLastError();
 }
-template <typename TS, typename TG, bool kDb>
-int bwd_typed(const NormBwdArgs& p, Shape sh, int most, cudaStream_t st) {
-  if (sh.threads == 32) {
-    if (sh.vec == 1) return bwd_go<TS, TG, kDb, 1, 8, false>(p, sh, most, st);
-    if (sh.nv == 1) return bwd_go<TS, TG, kDb, 8, 1, false>(p, sh, most, st);
-    if (sh.nv == 2) return bwd_go<TS, TG, kDb, 8, 2, false>(p, sh, most, st);
-    return bwd_go<TS, TG, kDb, 8, 3, false>(p, sh, most, st);
+template <typename TS, typename TG, bool kDb, bool kOdd>
+cudaError_t bwd_shaped(const NormBwdArgs& p, Shape sh, int most, int* parts, cudaStream_t st) {
+  if (sh.lanes == 8) return bwd_go<TS, TG, kDb, kOdd, 1, 8>(p, sh, most, parts, st);
+  if (sh.lanes == 16) return bwd_go<TS, TG, kDb, kOdd, 1, 16>(p, sh, most, parts, st);
+  if (sh.lanes == 32) {
+    if (sh.nv == 1) return bwd_go<TS, TG, kDb, kOdd, 1, 32>(p, sh, most, parts, st);
+    if (sh.nv == 2) return bwd_go<TS, TG, kDb, kOdd, 2, 32>(p, sh, most, parts, st);
+    return bwd_go<TS, TG, kDb, kOdd, 3, 32>(p, sh, most, parts, st);
   }
-  if (sh.vec == 1)
-    return sh.nv == 8 ? bwd_ring<TS, TG, 8>(p, sh, most, st) : bwd_ring<TS, TG, 16>(p, sh, most, st);
-  return bwd_go<TS, TG, kDb, 8, 2, true>(p, sh, most, st);
+  if (kOdd && sh.threads <= 256)
+    return bwd_go<TS, TG, kDb, kOdd, 2, 0, 256>(p, sh, most, parts, st);
+  return bwd_go<TS, TG, kDb, kOdd, 2, 0>(p, sh, most, parts, st);
+}
+template <typename TS, typename TG>
+cudaError_t bwd_typed(const NormBwdArgs& p, Shape sh, int most, int* parts, cudaStream_t st) {
+  if (sh.odd)
+    return p.db ? bwd_shaped<TS, TG, true, true>(p, sh, most, parts, st)
+                : bwd_shaped<TS, TG, false, true>(p, sh, most, parts, st);
+  return p.db ? bwd_shaped<TS, TG, true, false>(p, sh, most, parts, st)
+              : bwd_shaped<TS, TG, false, false>(p, sh, most, parts, st);
 }
 
 }  // namespace
 
 cudaError_t norm_fwd(const NormFwdArgs& p, cudaStream_t st) {
   const Shape sh = shape_of(p.width, true);
-  if (sh.threads == 0 || (sh.vec == 1 && sh.threads > 32 && ring_fwd(p) > kMaxRing)) {
+  if (sh.lanes < 0) {
     norm_fwd_rows<<<row_grid(p.rows), kThreads, 0, st>>>(p);
     return cudaGetLastError();
   }
@@ -845,31 +718,35 @@ cudaError_t norm_fwd(const NormFwdArgs& p, cudaStream_t st) {
   return p.res_f32 ? fwd_typed<bf16, float>(p, sh, st) : fwd_typed<bf16, bf16>(p, sh, st);
 }
 
-// The most partials of dw and db that a backward writes, whichever way it takes.
+// The most partials of dw and db that a backward writes, one a CTA: 16 warps an
+// SM (an odd width's rounded to its grid's multiple of 8).
 int norm_bwd_partials(long long rows, int width) {
-  (void)width;
-  return static_cast<int>(rows < kSms * kMaxResident ? rows : kSms * kMaxResident);
+  const Shape sh = shape_of(width, false);
+  const int resident = sh.lanes < 0 ? 2 : 512 / sh.threads;
+  const int cap = kSms * (resident < 1 ? 1 : resident) / 8 * 8;
+  return static_cast<int>(rows < cap ? rows : cap);
 }
 
 cudaError_t norm_bwd(const NormBwdArgs& p, cudaStream_t st) {
   const Shape sh = shape_of(p.width, false);
-  int parts = norm_bwd_partials(p.rows, p.width);
-  if (sh.threads && !(sh.vec == 1 && sh.threads > 32 && ring_bwd(p) > kMaxRing)) {
-    auto go = [&](auto ts, auto tg) {
-      parts = p.db ? bwd_typed<decltype(ts), decltype(tg), true>(p, sh, parts, st)
-                   : bwd_typed<decltype(ts), decltype(tg), false>(p, sh, parts, st);
-    };
-    if (p.s_f32) p.dy_f32 ? go(float{}, float{}) : go(float{}, bf16{});
-    else p.dy_f32 ? go(bf16{}, float{}) : go(bf16{}, bf16{});
+  const int most = norm_bwd_partials(p.rows, p.width);
+  int parts = most;
+  cudaError_t e;
+  if (sh.lanes >= 0) {
+    if (p.s_f32)
+      e = p.dy_f32 ? bwd_typed<float, float>(p, sh, most, &parts, st)
+                   : bwd_typed<float, bf16>(p, sh, most, &parts, st);
+    else
+      e = p.dy_f32 ? bwd_typed<bf16, float>(p, sh, most, &parts, st)
+                   : bwd_typed<bf16, bf16>(p, sh, most, &parts, st);
   } else {
-    const int want = static_cast<int>((p.rows + 31) / 32 < kMaxPartials ? (p.rows + 31) / 32
-                                                                        : kMaxPartials);
-    if (want < parts) parts = want;
+    const long long want = (p.rows + 31) / 32;
+    parts = static_cast<int>(want < most ? want : most);
     if (p.ds_a || p.ds_b) norm_bwd_rows<<<row_grid(p.rows), kThreads, 0, st>>>(p);
     if (p.dw || p.db)
       norm_bwd_cols<<<dim3((p.width + 31) / 32, parts), kColThreads, 0, st>>>(p, parts);
+    e = cudaGetLastError();
   }
-  cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess && (p.dw || p.db)) {
     norm_bwd_join<<<dim3((p.width + 31) / 32, p.db ? 2 : 1), kJoinWarps * 32, 0, st>>>(
         p.partial, p.dw, p.db, p.width, parts);

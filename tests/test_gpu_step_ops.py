@@ -152,6 +152,37 @@ def test_norm_sizes(rows, D, center):
         _check_norm(pkg, _norm_case(rows, D, center, dt, res, dt))
 
 
+@pytest.mark.parametrize("rows, D", [(20000, 13), (12001, 64), (9001, 101), (5000, 129), (4000, 257),
+                                     (3001, 513), (2000, 761), (2500, 775), (2501, 1030),
+                                     (1200, 4081), (1201, 4083), (700, 8177), (650, 8179),
+                                     (300, 8191), (40, 16370), (3, 16383)])
+def test_norm_ragged_widths(rows, D):
+    """Rows at every alignment, each CTA walking many of them, at the borders
+    between the ways a width is held."""
+    pkg = load_pkg()
+    _check_norm(pkg, _norm_case(rows, D, True, BF, FP, BF))
+    _check_norm(pkg, _norm_case(rows, D, False, FP, None, FP, bias=False))
+
+
+def test_norm_neighbours_stay_out():
+    """Infinities and NaN in a row stay in it, whatever shares its memory groups."""
+    pkg = load_pkg()
+    for D in (5, 100, 769, 1283):
+        c = _norm_case(24, D, True, FP, BF, FP)
+        clean, cg = _run_norm(pkg, c)
+        c["x"][7] = math.inf
+        c["x"][8, 0] = math.nan
+        c["dh"][11, -1] = math.nan
+        dirty, dg = _run_norm(pkg, c)
+        keep = [r for r in range(24) if r not in (7, 8)]
+        for a, b in zip(clean, dirty):
+            assert torch.equal(a[keep], b[keep])
+        assert torch.isnan(dirty[0][7]).all() and torch.isnan(dirty[0][8]).all()
+        keep.remove(11)
+        assert torch.equal(cg["x"][keep], dg["x"][keep])
+        assert torch.isnan(dg["x"][11, -1]) and not torch.isnan(dg["x"][11, :-1]).any()
+
+
 @pytest.mark.parametrize("x_dt", [BF, FP])
 @pytest.mark.parametrize("res_dt", [None, BF, FP])
 @pytest.mark.parametrize("out_dt", [BF, FP])
