@@ -155,7 +155,8 @@ def test_norm_sizes(rows, D, center):
 @pytest.mark.parametrize("rows, D", [(20000, 13), (12001, 64), (9001, 101), (5000, 129), (4000, 257),
                                      (3001, 513), (2000, 761), (2500, 775), (2501, 1030),
                                      (1200, 4081), (1201, 4083), (700, 8177), (650, 8179),
-                                     (300, 8191), (40, 16370), (3, 16383)])
+                                     (300, 8191), (40, 16370), (3, 16383),
+                                     (300, 16384), (320, 8200)])
 def test_norm_ragged_widths(rows, D):
     """Rows at every alignment, each CTA walking many of them, at the borders
     between the ways a width is held."""
