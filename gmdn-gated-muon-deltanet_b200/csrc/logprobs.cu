@@ -593,7 +593,6 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
     if (c0 + u * n + tid < chunks) c[u] = load(c0 + u * n + tid);
   const float4 st = __ldg(reinterpret_cast<const float4*>(p.stats) + r);
   const float m = st.x, ls = st.y, nan = __int_as_float(0x7fffffff);
-  const bool empty = ls == -INFINITY;
   const float gh = kEnt && p.g_entropy ? p.g_entropy[r] : 0.f;
   int t = -1;
   float gl = 0.f;
@@ -609,6 +608,7 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
   // alternative `tid`, on its way while the row is worked on
   int64_t top_i = -1;
   float top_g = 0.f;
+  bool any_top = false;
   if constexpr (kTop) {
     const int lane = tid & 31;
     const float* gk = p.g_top + r * p.top_k;
@@ -616,9 +616,15 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
       top_i = p.top_ids[r * p.top_k + tid];
       top_g = gk[tid];
     }
-    wsum += warp_sum((lane < p.top_k ? gk[lane] : 0.f) +
-                     (lane + 32 < p.top_k ? gk[lane + 32] : 0.f));
+    const float g0 = lane < p.top_k ? gk[lane] : 0.f;
+    const float g1 = lane + 32 < p.top_k ? gk[lane + 32] : 0.f;
+    any_top = g0 != 0.f || g1 != 0.f;   // NaN too
+    wsum += warp_sum(g0 + g1);
   }
+  // No gradient: a row without columns, and one whose cotangents are all 0 (an ignored target),
+  // whatever it holds.
+  const bool zero = ls == -INFINITY ||
+                    (gl == 0.f && gh == 0.f && !(kTop && __any_sync(~0u, any_top)));
   const float A = kEnt ? -fmaf(gh, st.z, wsum) : -wsum, B = -gh;
   auto grad2 = [&](float2 v) {
     float2 lp = __fadd2_rn(__fadd2_rn(v, pair(-m)), pair(-ls));
@@ -637,9 +643,9 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
     if (j >= chunks) break;
     float2 g[E / 2];
 #pragma unroll
-    for (int k = 0; k < E / 2; ++k) g[k] = empty ? pair(0.f) : grad2(c[u].get(k));
+    for (int k = 0; k < E / 2; ++k) g[k] = zero ? pair(0.f) : grad2(c[u].get(k));
     const int i0 = j * E - off;
-    if (j == tj && !empty) {
+    if (j == tj && !zero) {
 #pragma unroll
       for (int k = 0; k < E / 2; ++k) {
         if (i0 + 2 * k == t) g[k].x += gl;
@@ -669,7 +675,7 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
     const bool here = top_i >= max(c0 * E - off, 0) && top_i < min((c0 + n * U) * E - off, V);
     const float v = here ? grad2(pair(element(x + top_i))).x + top_g + (top_i == t ? gl : 0.f) : 0.f;
     __syncthreads();
-    if (here && !empty) out[top_i] = static_cast<T>(v);
+    if (here && !zero) out[top_i] = static_cast<T>(v);
   }
 }
 

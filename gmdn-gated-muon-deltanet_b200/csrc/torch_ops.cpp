@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <initializer_list>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -70,6 +71,24 @@ void check_f32(const char* op, const OptTensor& t, int64_t n) {
   TORCH_CHECK(!has(t) || (is_f32(*t) && t->numel() == n), op, ": expected ", n,
               " float32 values");
 }
+// Whether autograd has anything to record.
+bool any_requires_grad(std::initializer_list<const Tensor*> ts,
+                       std::initializer_list<const OptTensor*> opts) {
+  if (!c10::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->requires_grad()) return true;
+  for (const OptTensor* t : opts)
+    if (has(*t) && (*t)->requires_grad()) return true;
+  return false;
+}
+// In a plain backward (grad mode off) its op goes straight to the kernel, past the boxed
+// fallback that refuses second derivatives.
+struct BelowAutograd {
+  std::optional<at::AutoDispatchBelowADInplaceOrView> guard;
+  BelowAutograd() {
+    if (!c10::GradMode::is_enabled()) guard.emplace();
+  }
+};
 void* stream_of(const Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
 }
@@ -197,6 +216,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
                                          : at::zeros_like(s, s.options().dtype(dy_type));
     const OptTensor dh = res && grads[1].defined() ? OptTensor(grads[1]) : OptTensor();
     const bool need_x = flag("need_x"), need_res = flag("need_res");
+    const BelowAutograd below;
     auto [da, db, dw, dbias] =
         norm_bwd_op(s, saved[1], w.defined() ? OptTensor(w) : OptTensor(), dy, dh, flag("center"),
                     (need_x && !x_f32) || (need_res && !res_f32),
@@ -209,6 +229,10 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
 
 Norm norm_fwd_autograd(const Tensor& x, const OptTensor& res, const OptTensor& w,
                        const OptTensor& b, double eps, bool center, bool out_f32) {
+  if (!any_requires_grad({&x}, {&res, &w, &b})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return norm_fwd_op(x, res, w, b, eps, center, out_f32);
+  }
   auto r = NormFunction::apply(x, res, w, b, eps, center, out_f32);
   return {r[0], r[1], r[2]};
 }
@@ -372,6 +396,7 @@ struct LogprobsFunction : torch::autograd::Function<LogprobsFunction> {
     auto cot = [&](int i, bool used) {
       return used && grads[i].defined() ? OptTensor(grads[i].to(at::kFloat)) : OptTensor();
     };
+    const BelowAutograd below;
     Tensor g = token_logprobs_bwd_op(
         saved[0], opt(saved[1]), opt(saved[2]), saved[3], cot(0, saved[1].defined()),
         cot(1, ctx->saved_data["entropy"].toBool()), cot(2, ctx->saved_data["top_k"].toInt() > 0),
@@ -382,6 +407,10 @@ struct LogprobsFunction : torch::autograd::Function<LogprobsFunction> {
 
 Logprobs token_logprobs_fwd_autograd(const Tensor& logits, const OptTensor& targets, bool entropy,
                                      int64_t top_k, int64_t ignore_index) {
+  if (!any_requires_grad({&logits}, {})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return token_logprobs_fwd_op(logits, targets, entropy, top_k, ignore_index);
+  }
   auto r = LogprobsFunction::apply(logits, targets, entropy, top_k, ignore_index);
   return {r[0], r[1], r[2], r[3], r[4]};
 }
@@ -512,9 +541,11 @@ TORCH_LIBRARY_IMPL(gmdn, Autograd, m) {
   m.impl("norm_fwd", norm_fwd_autograd);
   m.impl("token_logprobs_fwd", token_logprobs_fwd_autograd);
   // no derivative: a second one through these raises
-  for (const char* name : {"norm_bwd", "token_logprobs_bwd", "pack8", "unpack8", "act8_fwd",
-                           "act8_bwd"})
+  for (const char* name : {"norm_bwd", "token_logprobs_bwd"})
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
+  // checkpoints: autograd does not see them
+  for (const char* name : {"pack8", "unpack8", "act8_fwd", "act8_bwd"})
+    m.impl(name, torch::CppFunction::makeFallthrough());
 }
 
 }  // namespace

@@ -38,6 +38,10 @@ __all__ = ["layer_norm", "rms_norm", "token_logprobs", "TokenLogprobs", "pack8",
 
 load_torch_ops()
 _ops = torch.ops.gmdn
+_norm_fwd = _ops.norm_fwd.default
+_token_logprobs_fwd = _ops.token_logprobs_fwd.default
+_pack8, _unpack8 = _ops.pack8.default, _ops.unpack8.default
+_act8_fwd, _act8_bwd = _ops.act8_fwd.default, _ops.act8_bwd.default
 MAX_TOP_K = 64
 BLOCK8 = 128   # consecutive elements that share a scale
 
@@ -98,9 +102,11 @@ def _norm(name: str, center: bool, x: Tensor, weight: Optional[Tensor], bias: Op
         raise TypeError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
     _same_device(name, x, weight, bias, residual)
     # the parameters' casts are differentiable: their gradients come back in their own types
-    y, h, _ = _ops.norm_fwd.default(x, residual, None if weight is None else weight.float(),
-                                    None if bias is None else bias.float(), float(eps), center,
-                                    out_dtype == torch.float32)
+    if weight is not None and weight.dtype != torch.float32:
+        weight = weight.float()
+    if bias is not None and bias.dtype != torch.float32:
+        bias = bias.float()
+    y, h, _ = _norm_fwd(x, residual, weight, bias, eps, center, out_dtype == torch.float32)
     return y if residual is None else (y, h)
 
 
@@ -167,7 +173,8 @@ def token_logprobs(logits: Tensor, targets: Optional[Tensor] = None, *, entropy:
     ``logits[:, :-1]`` or the live columns of a padded head is read in place).
     targets: (...) int64 or int32, or None for no log probabilities; a target
     equal to ignore_index gives 0 and no gradient, any other outside [0, V)
-    gives NaN.  entropy: also the entropy of each row's distribution.  top_k:
+    gives NaN.  A row whose cotangents are all 0 has a zero gradient whatever it
+    holds.  entropy: also the entropy of each row's distribution.  top_k:
     also the log probabilities and columns of the top_k (at most 64) largest
     logits, falling, ties to the lowest column.
 
@@ -193,8 +200,8 @@ def token_logprobs(logits: Tensor, targets: Optional[Tensor] = None, *, entropy:
     _same_device("token_logprobs", logits, targets)
     if targets is not None and targets.dtype == torch.int32:
         targets = targets.long()
-    lp, ent, tops, ids, _ = _ops.token_logprobs_fwd.default(logits, targets, bool(entropy),
-                                                            int(top_k), int(ignore_index))
+    lp, ent, tops, ids, _ = _token_logprobs_fwd(logits, targets, bool(entropy), int(top_k),
+                                                int(ignore_index))
     return TokenLogprobs(None if targets is None else lp, ent if entropy else None,
                          tops if top_k else None, ids if top_k else None)
 
@@ -249,6 +256,8 @@ def _check_packed(name: str, p: Packed8) -> None:
     if p.codes.dtype != torch.int8 or p.scales.dtype != torch.float32:
         raise TypeError(f"{name}: codes must be int8 and scales float32, got {p.codes.dtype} and "
                         f"{p.scales.dtype}")
+    if p.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{name}: a checkpoint comes back in bfloat16 or float32, not {p.dtype}")
     if p.scales.dim() != 1 or p.scales.numel() != (p.codes.numel() + BLOCK8 - 1) // BLOCK8:
         raise ValueError(f"{name}: {tuple(p.codes.shape)} codes need one scale for each {BLOCK8} "
                          f"elements, got {tuple(p.scales.shape)}")
@@ -262,14 +271,14 @@ def pack8(x: Tensor) -> Packed8:
     infinity as NaN.  Not differentiable: the result is a checkpoint."""
     _f32_flag(x, "x")
     _require_cuda("pack8", x)
-    return Packed8(*_ops.pack8.default(x.detach()), x.dtype)
+    return Packed8(*_pack8(x.detach()), x.dtype)
 
 
 def unpack8(packed: Packed8) -> Tensor:
     """The tensor that ``pack8`` kept, in its shape and type."""
     _check_packed("unpack8", packed)
     _same_device("unpack8", packed.codes, packed.scales)
-    return _ops.unpack8.default(packed.codes, packed.scales, packed.dtype == torch.float32)
+    return _unpack8(packed.codes, packed.scales, packed.dtype == torch.float32)
 
 
 def act8_forward(x: Tensor, gate: Optional[Tensor] = None) -> tuple[Tensor, Act8Saved]:
@@ -281,7 +290,7 @@ def act8_forward(x: Tensor, gate: Optional[Tensor] = None) -> tuple[Tensor, Act8
         raise ValueError(f"gate must be like x, {tuple(x.shape)} {x.dtype}, got "
                          f"{tuple(gate.shape)} {gate.dtype}")
     _same_device("act8_forward", x, gate)
-    y, codes, scales, gcodes, gscales = _ops.act8_fwd.default(
+    y, codes, scales, gcodes, gscales = _act8_fwd(
         x.detach(), None if gate is None else gate.detach())
     return y, Act8Saved(Packed8(codes, scales, x.dtype),
                         None if gate is None else Packed8(gcodes, gscales, x.dtype))
@@ -303,7 +312,7 @@ def act8_backward(saved: Act8Saved, dy: Tensor, restore: bool = True):
             raise ValueError("act8_backward: the gate's checkpoint is not like the input's")
     parts = [x.codes, x.scales] + ([None, None] if gate is None else [gate.codes, gate.scales])
     _same_device("act8_backward", dy, *parts)
-    dx, dgate, y = _ops.act8_bwd.default(*parts, dy.detach(), bool(restore))
+    dx, dgate, y = _act8_bwd(*parts, dy.detach(), bool(restore))
     return dx, dgate if gate is not None else None, y if restore else None
 
 

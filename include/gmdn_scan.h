@@ -275,7 +275,8 @@ int gmdn_token_logprobs_fwd(const void* logits, const int64_t* targets, float* l
 
 /* Backward: dlogits (batch, length, vocab) contiguous, in the logits' type,
  * from the cotangents of logprobs, entropy (rows) and top_logprobs (rows,
- * top_k), each of which may be NULL. */
+ * top_k), each of which may be NULL.  A row whose cotangents are all 0 (an
+ * ignored target) gets zeros whatever it holds. */
 int gmdn_token_logprobs_bwd(const void* logits, const int64_t* targets, const float* stats,
                             const int64_t* top_ids, const float* g_logprobs,
                             const float* g_entropy, const float* g_top, void* dlogits,

@@ -433,6 +433,32 @@ def test_logprobs_bad_rows_and_targets():
     assert torch.equal(lp, torch.zeros(6, device="cuda"))
 
 
+def test_logprobs_ignored_rows_have_no_gradient():
+    """Padded positions may hold anything: their cotangents are 0, so is their
+    gradient, and the other rows do not see them."""
+    pkg = load_pkg()
+    for V in (100, 5001):
+        z = _logits(6, V, BF)
+        t = torch.tensor([1, -100, 2, -100, -100, 3])
+        clean = z.cuda().requires_grad_(True)
+        (want,) = torch.autograd.grad(pkg.token_logprobs(clean, t.cuda()).logprobs.sum(), clean)
+        z[1] = math.nan
+        z[3, 5] = math.inf
+        z[4] = -math.inf
+        zg = z.cuda().requires_grad_(True)
+        got = pkg.token_logprobs(zg, t.cuda(), top_k=3)
+        (g,) = torch.autograd.grad([got.logprobs, got.top_logprobs], zg,
+                                   [torch.ones(6, device="cuda"), torch.zeros(6, 3, device="cuda")])
+        assert torch.equal(g, want)
+        assert torch.equal(g[[1, 3, 4]], torch.zeros_like(g[:3]))
+        # a cotangent on an alternative of such a row is not lost
+        got = pkg.token_logprobs(zg, t.cuda(), top_k=3)
+        cot = torch.zeros(6, 3, device="cuda")
+        cot[1, 2] = 1.0
+        (g,) = torch.autograd.grad(got.top_logprobs, zg, cot)
+        assert torch.isnan(g[1]).all() and not torch.isnan(g[2:]).any()
+
+
 @pytest.mark.parametrize("dtype", [BF, FP])
 @pytest.mark.parametrize("V", [64, 1001, 32000])
 def test_logprobs_views(dtype, V):
@@ -785,6 +811,63 @@ def test_operators_in_a_captured_graph(dt):
             assert (a - b).norm() <= 1e-5 * b.norm()
         else:
             assert torch.equal(a, b), n
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams share nothing."""
+    pkg = load_pkg()
+    p, idx, t = _params(BF, V=5003)
+    leaves = [n for n in p if n != "dt"]
+    gp = {n: p[n].cuda().requires_grad_(True) if n != "dt" else BF for n in p}
+    idx, t = idx.cuda(), t.cuda()
+    shifted = (t + 7) % 5003
+
+    def step(targets):
+        loss, got = _block(pkg, gp, idx, targets)
+        return (loss.detach(), got.top_ids,
+                *torch.autograd.grad(loss, [gp[n] for n in leaves if n != "emb"]))
+
+    want = [step(t), step(shifted)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        got = [None, None]
+        for i, (s, targets) in enumerate(zip(streams, (t, shifted))):
+            with torch.cuda.stream(s):
+                got[i] = step(targets)
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_the_same_tensor_twice_and_nothing_at_all():
+    pkg = load_pkg()
+    x = torch.randn(9, 200, generator=_gen(1)).cuda().requires_grad_(True)
+    w = torch.randn(200, generator=_gen(2)).cuda().requires_grad_(True)
+    y, h = pkg.rms_norm(x, w, w, 1e-5, residual=x)      # x + x, and w as weight and bias
+    cot = torch.randn(9, 200, generator=_gen(3)).cuda()
+    gx, gw = torch.autograd.grad([y, h], [x, w], [cot, cot])
+    xr, wr = x.detach().double().requires_grad_(True), w.detach().double().requires_grad_(True)
+    yr, hr = so.norm(2 * xr, wr, wr, 1e-5, None, False)
+    ex, ew = torch.autograd.grad([yr, hr], [xr, wr], [cot.double()] * 2)
+    # fp32 through sums of 200 and of 9
+    assert (gx - ex).abs().max() < 64 * EPS * ex.abs().max()
+    assert (gw - ew).abs().max() < 64 * EPS * ew.abs().max()
+    a = _acts(1000, BF).cuda()
+    y, saved = pkg.act8_forward(a, a)
+    _within(y, so.act(a.cpu(), a.cpu()), (U(BF) + 2.0 ** -20) * so.act(a.cpu(), a.cpu()).abs(), "y")
+    for shape in ((0, 16), (3, 0, 16)):
+        x = torch.empty(shape, device="cuda", requires_grad=True)
+        w1 = torch.randn(32, 16, device="cuda", requires_grad=True)
+        w2 = torch.randn(8, 32, device="cuda", requires_grad=True)
+        out = pkg.mlp8(x, w1, w2, w1)
+        out.sum().backward()
+        assert out.shape == (*shape[:-1], 8) and x.grad.shape == x.shape
+        assert not w1.grad.any() and not w2.grad.any()
+    empty = torch.empty(0, 5, device="cuda")
+    y, saved = pkg.act8_forward(empty, empty)
+    dx, dgate, back = pkg.act8_backward(saved, empty)
+    assert y.shape == dx.shape == dgate.shape == back.shape == (0, 5)
 
 
 def test_opcheck():

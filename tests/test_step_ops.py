@@ -55,6 +55,8 @@ def test_refuses_cpu_tensors():
     (lambda p, x: p.unpack8(p.Packed8(x, torch.zeros(1), torch.float32)), TypeError),
     (lambda p, x: p.unpack8(p.Packed8(torch.zeros(129, dtype=torch.int8), torch.zeros(1),
                                       torch.float32)), ValueError),
+    (lambda p, x: p.unpack8(p.Packed8(torch.zeros(4, dtype=torch.int8), torch.zeros(1),
+                                      torch.float16)), TypeError),
     (lambda p, x: p.act8_backward(p.Act8Saved(p.Packed8(torch.zeros(4, 16, dtype=torch.int8),
                                                         torch.zeros(1), torch.float32), None),
                                   x.bfloat16()), ValueError),
