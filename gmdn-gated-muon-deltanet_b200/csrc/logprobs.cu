@@ -529,6 +529,7 @@ __global__ void __launch_bounds__(kMaxThreads) logprobs_fwd_kernel(LogprobArgs p
 // ---------------------------------------------------------------------------
 
 constexpr int kBwdThreads = 256;   // at most; at least kMaxTopK
+constexpr int kBwdUnroll = 4;
 
 // Elements i0 .. i0 + E - 1 of a row that lies `shift` elements above a 16-byte
 // boundary there: the two aligned chunks that hold them, shifted together.
@@ -565,10 +566,12 @@ __device__ __forceinline__ Chunk<T> load_shifted(const T* x, int i0, int shift) 
 // the end, each by one thread.
 template <typename T, bool kEnt, bool kTop>
 __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p, int parts) {
-  constexpr int E = Chunk<T>::E, U = 4;
-  const long long r = blockIdx.x / parts;
-  const int part = static_cast<int>(blockIdx.x - r * parts), tid = threadIdx.x, n = blockDim.x;
-  const long long b = r / p.length;
+  constexpr int E = Chunk<T>::E, U = kBwdUnroll;
+  // 32-bit divisions: the grid has fewer than 2^31 CTAs, so there are fewer rows than that
+  const uint32_t ru = blockIdx.x / static_cast<uint32_t>(parts);
+  const uint32_t b = ru / static_cast<uint32_t>(p.length);
+  const long long r = ru;
+  const int part = static_cast<int>(blockIdx.x - ru * parts), tid = threadIdx.x, n = blockDim.x;
   const T* x = static_cast<const T*>(p.logits) + b * p.stride_b + (r - b * p.length) * p.stride_t;
   T* out = static_cast<T*>(p.dlogits) + r * p.vocab;
   const int V = p.vocab;
@@ -578,7 +581,10 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
   const int shift =
       static_cast<int>((reinterpret_cast<uintptr_t>(x) / sizeof(T) + E - off) % E);
   const int c0 = part * n * U;
-  auto load = [&](int j) {
+  // chunks of `out` that lie wholly in the row; with shift 0 those of the logits too
+  const int full0 = off ? 1 : 0, full1 = (off + V) / E;
+  uint4* out16 = reinterpret_cast<uint4*>(out - off);
+  auto load_edge = [&](int j) {
     const int i0 = j * E - off;
     if (i0 - shift >= 0 && i0 - shift + (shift ? 2 * E : E) <= V) return load_shifted(x, i0, shift);
     Chunk<T> c;
@@ -588,9 +594,26 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
     return c;
   };
   Chunk<T> c[U];
+  if (shift == 0) {
+    const uint4* in16 = reinterpret_cast<const uint4*>(x - off);
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (c0 + u * n + tid < chunks) c[u] = load(c0 + u * n + tid);
+    for (int u = 0; u < U; ++u) {
+      const int j = c0 + u * n + tid;
+      if (j >= full0 && j < full1) {
+        const uint4 v = __ldcs(in16 + j);
+        c[u].w[0] = v.x;
+        c[u].w[1] = v.y;
+        c[u].w[2] = v.z;
+        c[u].w[3] = v.w;
+      } else if (j < chunks) {
+        c[u] = load_edge(j);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * n + tid < chunks) c[u] = load_edge(c0 + u * n + tid);
+  }
   const float4 st = __ldg(reinterpret_cast<const float4*>(p.stats) + r);
   const float m = st.x, ls = st.y, nan = __int_as_float(0x7fffffff);
   const float gh = kEnt && p.g_entropy ? p.g_entropy[r] : 0.f;
@@ -643,16 +666,20 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
     if (j >= chunks) break;
     float2 g[E / 2];
 #pragma unroll
-    for (int k = 0; k < E / 2; ++k) g[k] = zero ? pair(0.f) : grad2(c[u].get(k));
-    const int i0 = j * E - off;
-    if (j == tj && !zero) {
+    for (int k = 0; k < E / 2; ++k) g[k] = pair(0.f);
+    if (!zero) {
 #pragma unroll
-      for (int k = 0; k < E / 2; ++k) {
-        if (i0 + 2 * k == t) g[k].x += gl;
-        if (i0 + 2 * k + 1 == t) g[k].y += gl;
+      for (int k = 0; k < E / 2; ++k) g[k] = grad2(c[u].get(k));
+      if (j == tj) {
+        const int at = t + off - j * E;
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) {
+          if (2 * k == at) g[k].x += gl;
+          if (2 * k + 1 == at) g[k].y += gl;
+        }
       }
     }
-    if (i0 >= 0 && i0 + E <= V) {
+    if (j >= full0 && j < full1) {
       uint4 o;
       if constexpr (sizeof(T) == 2) {
         __nv_bfloat162 h[4];
@@ -663,8 +690,9 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
         o = make_uint4(__float_as_uint(g[0].x), __float_as_uint(g[0].y), __float_as_uint(g[1].x),
                        __float_as_uint(g[1].y));
       }
-      *reinterpret_cast<uint4*>(out + i0) = o;
+      out16[j] = o;
     } else {
+      const int i0 = j * E - off;
 #pragma unroll
       for (int k = 0; k < E; ++k)
         if (i0 + k >= 0 && i0 + k < V)
@@ -721,8 +749,9 @@ template <typename T, bool kEnt, bool kTop>
 cudaError_t launch_bwd(const LogprobArgs& p, cudaStream_t st) {
   const long long rows = p.batch * p.length;
   const int chunks = (p.vocab * static_cast<long long>(sizeof(T)) + 15) / 16 + 1;
-  const int threads = chunks >= 4 * 256 ? 256 : (chunks >= 4 * 128 ? 128 : 64);
-  const int parts = (chunks + threads * 4 - 1) / (threads * 4);
+  constexpr int U = kBwdUnroll;
+  const int threads = chunks >= U * 256 ? 256 : (chunks >= U * 128 ? 128 : 64);
+  const int parts = (chunks + threads * U - 1) / (threads * U);
   if (rows * parts > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   logprobs_bwd_kernel<T, kEnt, kTop>
       <<<static_cast<unsigned>(rows * parts), threads, 0, st>>>(p, parts);
