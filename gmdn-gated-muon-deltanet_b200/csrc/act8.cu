@@ -13,6 +13,12 @@
 //   SwiGLU: y = a sig(a) u;  du = dy a sig(a),  da = dy u sig(a) (1 + a (1 - sig(a)))
 // with the restored x, (u, a) in the backward, which also writes the restored
 // y: the weight gradient of the projection that read y needs it.
+//
+// Memory bounds it, with the instruction slots close: bf16 GELU moves 5 bytes an
+// element forward and 7 backward, which leaves ~27 and ~38 instructions an
+// element at the copy rate; the kernels take 19.  Measured (B200): 16384 x 4096
+// bf16 GELU 60 us forward (0.86 of the 6536 GB/s copy rate) and 86 backward
+// (0.84), SwiGLU at 0.88 and more; fp32 GELU at 0.54 and 0.68 (normcdff).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

