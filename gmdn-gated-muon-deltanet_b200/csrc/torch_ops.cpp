@@ -185,22 +185,21 @@ NormGrads norm_bwd_op(const Tensor& s, const Tensor& stats, const OptTensor& w, 
 }
 
 struct NormFunction : torch::autograd::Function<NormFunction> {
+  // one saved word: the map of saved data costs more than the values
+  enum : int64_t { kCenter = 1, kOutF32 = 2, kXF32 = 4, kRes = 8, kResF32 = 16, kNeedX = 32,
+                   kNeedRes = 64, kNeedW = 128, kNeedB = 256 };
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& res,
                                const OptTensor& w, const OptTensor& b, double eps, bool center,
                                bool out_f32) {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [y, h, stats] = norm_fwd_op(x, res, w, b, eps, center, out_f32);
     auto wants = [](const OptTensor& t) { return has(t) && t->requires_grad(); };
-    ctx->saved_data["center"] = center;
-    ctx->saved_data["out_f32"] = out_f32;
-    ctx->saved_data["x_f32"] = is_f32(x);
-    ctx->saved_data["res"] = has(res);
-    ctx->saved_data["res_f32"] = has(res) && is_f32(*res);
-    // (needs_input_grad would count only defined inputs)
-    ctx->saved_data["need_x"] = x.requires_grad();
-    ctx->saved_data["need_res"] = wants(res);
-    ctx->saved_data["need_w"] = wants(w);
-    ctx->saved_data["need_b"] = wants(b);
+    const int64_t flags = (center ? kCenter : 0) | (out_f32 ? kOutF32 : 0) |
+                          (is_f32(x) ? kXF32 : 0) | (has(res) ? kRes : 0) |
+                          (has(res) && is_f32(*res) ? kResF32 : 0) |
+                          (x.requires_grad() ? kNeedX : 0) | (wants(res) ? kNeedRes : 0) |
+                          (wants(w) ? kNeedW : 0) | (wants(b) ? kNeedB : 0);
+    ctx->saved_data["flags"] = flags;
     ctx->save_for_backward({has(res) ? h : x, stats, has(w) ? *w : Tensor()});
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable(has(res) ? variable_list{stats} : variable_list{h, stats});
@@ -208,21 +207,22 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    auto flag = [&](const char* name) { return ctx->saved_data[name].toBool(); };
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    auto flag = [flags](int64_t f) { return (flags & f) != 0; };
     const Tensor &s = saved[0], &w = saved[2];
-    const bool res = flag("res"), x_f32 = flag("x_f32"), res_f32 = flag("res_f32");
-    const auto dy_type = flag("out_f32") ? at::kFloat : at::kBFloat16;
+    const bool res = flag(kRes), x_f32 = flag(kXF32), res_f32 = flag(kResF32);
+    const auto dy_type = flag(kOutF32) ? at::kFloat : at::kBFloat16;
     const Tensor dy = grads[0].defined() ? grads[0].to(dy_type)
                                          : at::zeros_like(s, s.options().dtype(dy_type));
     const OptTensor dh = res && grads[1].defined() ? OptTensor(grads[1]) : OptTensor();
-    const bool need_x = flag("need_x"), need_res = flag("need_res");
+    const bool need_x = flag(kNeedX), need_res = flag(kNeedRes);
     const BelowAutograd below;
     auto [da, db, dw, dbias] =
-        norm_bwd_op(s, saved[1], w.defined() ? OptTensor(w) : OptTensor(), dy, dh, flag("center"),
+        norm_bwd_op(s, saved[1], w.defined() ? OptTensor(w) : OptTensor(), dy, dh, flag(kCenter),
                     (need_x && !x_f32) || (need_res && !res_f32),
-                    (need_x && x_f32) || (need_res && res_f32), flag("need_w"), flag("need_b"));
+                    (need_x && x_f32) || (need_res && res_f32), flag(kNeedW), flag(kNeedB));
     return {need_x ? (x_f32 ? db : da) : Tensor(), need_res ? (res_f32 ? db : da) : Tensor(),
-            flag("need_w") ? dw : Tensor(), flag("need_b") ? dbias : Tensor(),
+            flag(kNeedW) ? dw : Tensor(), flag(kNeedB) ? dbias : Tensor(),
             Tensor(), Tensor(), Tensor()};
   }
 };
