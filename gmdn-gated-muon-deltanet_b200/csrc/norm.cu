@@ -19,7 +19,7 @@
 // thread's rows.  Measured (B200, copy rate 6536 GB/s): 16384 x 768, fp32 stream
 // and bf16 branch: forward 26 us (0.90 of the copy rate), backward 42 us (0.73,
 // with the 5 us join of the CTAs' column sums); 8192 x 4096 and wider fp32 rows
-// 0.87 to 0.92 both ways; 8192 x 8192 bf16 109 and 112 us (0.75, 0.73).
+// 0.87 to 0.92 both ways; 8192 x 8192 bf16 96 and 112 us (0.86, 0.73).
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -103,39 +103,28 @@ __device__ __forceinline__ void store_group(void* base, size_t i, const float* v
 }
 
 // Sums over a row's threads; every thread gets them.  LPR lanes of a warp a row,
-// or (0) a CTA: one barrier, `red` alternating between two buffers of 64
-// floats, so that a warp that is ahead writes the other one.
+// or (0) a CTA: one barrier for N sums (at most 4), `red` alternating between
+// two buffers of 128 floats, so that a warp that is ahead writes the other one.
 template <int LPR>
 __device__ __forceinline__ float lane_sum(float v) {
 #pragma unroll
   for (int o = (LPR ? LPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   return v;
 }
-template <int LPR>
-__device__ __forceinline__ void row_sum(float& a, float*& red) {
-  a = lane_sum<LPR>(a);
-  if constexpr (LPR == 0) {
-    const int lane = threadIdx.x & 31, n = blockDim.x >> 5;
-    if (lane == 0) red[threadIdx.x >> 5] = a;
-    __syncthreads();
-    a = warp_sum(lane < n ? red[lane] : 0.f);
-    red = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(red) ^ 256);
-  }
-}
-template <int LPR>
-__device__ __forceinline__ void row_sums(float& a, float& b, float*& red) {
-  a = lane_sum<LPR>(a);
-  b = lane_sum<LPR>(b);
+template <int LPR, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float*& red) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = lane_sum<LPR>(v[i]);
   if constexpr (LPR == 0) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, n = blockDim.x >> 5;
     if (lane == 0) {
-      red[w] = a;
-      red[32 + w] = b;
+#pragma unroll
+      for (int i = 0; i < N; ++i) red[32 * i + w] = v[i];
     }
     __syncthreads();
-    a = warp_sum(lane < n ? red[lane] : 0.f);
-    b = warp_sum(lane < n ? red[32 + lane] : 0.f);
-    red = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(red) ^ 256);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < n ? red[32 * i + lane] : 0.f);
+    red = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(red) ^ 512);
   }
 }
 
@@ -223,14 +212,15 @@ struct Place {
   }
 };
 
-template <typename TX, typename TR, int NV, int LPR, bool kOdd>
-__global__ void __launch_bounds__(LPR ? kRowThreads : kMaxCta,
-                                  LPR == 0 && NV == 2 && !kOdd && sizeof(TX) + sizeof(TR) < 8 ? 2 : 1)
-norm_fwd_regs(NormFwdArgs p) {
+// R rows a step: their sums share barriers and their loads of the weights.  CTA
+// rows with two groups a thread take two (8192 x 8192 bf16 layer norm: 96 us
+// against 109 one row a step, two CTAs an SM instead of one).
+template <typename TX, typename TR, int NV, int LPR, bool kOdd, int R>
+__global__ void __launch_bounds__(LPR ? kRowThreads : kMaxCta) norm_fwd_regs(NormFwdArgs p) {
   constexpr bool kRes = !std::is_same<TR, None>::value;
   using TL = typename std::conditional<kRes, TR, TX>::type;   // the residual's loads
   constexpr bool kHf32 = std::is_same<TX, float>::value || std::is_same<TR, float>::value;
-  __shared__ __align__(512) float buf[128];
+  __shared__ __align__(1024) float buf[256];
   extern __shared__ __align__(16) float params[];   // kOdd: weight, bias, a copy a slot
   float* red = buf;
   const int D = p.width;
@@ -248,96 +238,104 @@ norm_fwd_regs(NormFwdArgs p) {
   }
   const TX* x = static_cast<const TX*>(p.x);
   const TL* res = static_cast<const TL*>(p.res);
-  Raw<TX> rx[NV];
-  Raw<TL> rr[NV];
-  auto fetch = [&](long long row) {
-    if (row >= p.rows) return;
-    const size_t base = at.base(row, D);
+  Raw<TX> rx[R][NV];
+  Raw<TL> rr[R][NV];
+  auto fetch = [&](long long first) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
-      if (at.has(v)) {
-        at.load(rx[v], x, base + at.group(v) * 8, total);
-        if constexpr (kRes) at.load(rr[v], res, base + at.group(v) * 8, total);
+    for (int q = 0; q < R; ++q) {
+      const long long row = first + q * at.step;
+      if (row < p.rows) {
+        const size_t base = at.base(row, D);
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+          if (at.has(v)) {
+            at.load(rx[q][v], x, base + at.group(v) * 8, total);
+            if constexpr (kRes) at.load(rr[q][v], res, base + at.group(v) * 8, total);
+          }
       }
+    }
   };
   fetch(at.row);
   // a warp's rows go together: its lanes meet in the sums whether they have a row or not
-  for (long long r = at.row; r - at.lead < p.rows; r += at.step) {
-    const bool live = LPR == 0 || LPR == 32 || r < p.rows;
-    const size_t base = at.base(r, D);
-    float s[NV][8], sum = 0.f;
+  for (long long r = at.row; r - at.lead < p.rows; r += R * at.step) {
+    float s[R][NV][8], sum[R], mean[R], d12[2 * R], rstd[R];
+    auto live = [&](int q) {
+      return (q == 0 && (LPR == 0 || LPR == 32)) || r + q * at.step < p.rows;
+    };
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const bool in = at.has(v) && live;
+    for (int q = 0; q < R; ++q) {
+      sum[q] = mean[q] = d12[2 * q] = d12[2 * q + 1] = 0.f;
+      const size_t base = at.base(r + q * at.step, D);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        s[v][k] = 0.f;
-        if (in && (!kOdd || at.bits(v) >> k & 1)) {
-          s[v][k] = rx[v].get(k);
-          if constexpr (kRes) s[v][k] += rr[v].get(k);
+      for (int v = 0; v < NV; ++v) {
+        const bool in = at.has(v) && live(q);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          s[q][v][k] = 0.f;
+          if (in && (!kOdd || at.bits(v) >> k & 1)) {
+            s[q][v][k] = rx[q][v].get(k);
+            if constexpr (kRes) s[q][v][k] += rr[q][v].get(k);
+          }
         }
-      }
-      if constexpr (kRes && !kHf32) round_bf16(s[v]);
+        if constexpr (kRes && !kHf32) round_bf16(s[q][v]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum += s[v][k];
-      if constexpr (kRes)
-        if (in) store_group(p.h, base + at.group(v) * 8, s[v], kHf32, at.bits(v));
+        for (int k = 0; k < 8; ++k) sum[q] += s[q][v][k];
+        if constexpr (kRes)
+          if (in) store_group(p.h, base + at.group(v) * 8, s[q][v], kHf32, at.bits(v));
+      }
     }
-    fetch(r + at.step);
-    float mean = 0.f;
+    fetch(r + R * at.step);
     if (p.center) {
-      row_sum<LPR>(sum, red);
-      mean = sum * inv;
+      row_sums<LPR>(sum, red);
+#pragma unroll
+      for (int q = 0; q < R; ++q) mean[q] = sum[q] * inv;
     }
-    float d1 = 0.f, d2 = 0.f;
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        if (at.has(v)) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float d = !kOdd || at.bits(v) >> k & 1 ? s[q][v][k] - mean[q] : 0.f;
+            d12[2 * q] += d;
+            d12[2 * q + 1] = fmaf(d, d, d12[2 * q + 1]);
+          }
+        }
+    row_sums<LPR>(d12, red);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      float d1 = d12[2 * q], d2 = d12[2 * q + 1] * inv;
+      if (p.center) {   // what the rounding of the mean left, taken out of both
+        d1 *= inv;
+        mean[q] += d1;
+        d2 = fmaxf(d2 - d1 * d1, 0.f);
+      }
+      rstd[q] = rsqrtf(d2 + p.eps);
+      if (at.tid == 0 && live(q)) {
+        p.rstd[r + q * at.step] = rstd[q];
+        if (p.center) p.mean[r + q * at.step] = mean[q];
+      }
+    }
 #pragma unroll
     for (int v = 0; v < NV; ++v)
       if (at.has(v)) {
-        if (!at.whole(v)) {
+        float w[8], b[8];
+        if (p.weight) at.param(p.weight, sw, v, w);
+        if (p.bias) at.param(p.bias, sb, v, b);
+#pragma unroll
+        for (int q = 0; q < R; ++q) {
+          if (!live(q)) continue;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float d = at.bits(v) >> k & 1 ? s[v][k] - mean : 0.f;
-            d1 += d;
-            d2 = fmaf(d, d, d2);
+            float y = (s[q][v][k] - mean[q]) * rstd[q];
+            if (p.weight) y *= w[k];
+            if (p.bias) y += b[k];
+            s[q][v][k] = y;
           }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float d = s[v][k] - mean;
-            d1 += d;
-            d2 = fmaf(d, d, d2);
-          }
+          store_group(p.y, at.base(r + q * at.step, D) + at.group(v) * 8, s[q][v], p.y_f32,
+                      at.bits(v));
         }
-      }
-    row_sums<LPR>(d1, d2, red);
-    d2 *= inv;
-    if (p.center) {   // what the rounding of the mean left, taken out of both
-      d1 *= inv;
-      mean += d1;
-      d2 = fmaxf(d2 - d1 * d1, 0.f);
-    }
-    const float rstd = rsqrtf(d2 + p.eps);
-    if (at.tid == 0 && live) {
-      p.rstd[r] = rstd;
-      if (p.center) p.mean[r] = mean;
-    }
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-      if (at.has(v) && live) {
-        float q[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) s[v][k] = (s[v][k] - mean) * rstd;
-        if (p.weight) {
-          at.param(p.weight, sw, v, q);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) s[v][k] *= q[k];
-        }
-        if (p.bias) {
-          at.param(p.bias, sb, v, q);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) s[v][k] += q[k];
-        }
-        store_group(p.y, base + at.group(v) * 8, s[v], p.y_f32, at.bits(v));
       }
   }
 }
@@ -349,7 +347,7 @@ norm_fwd_regs(NormFwdArgs p) {
 template <typename TS, typename TG, int NV, int LPR, bool kOdd, bool kDb, int kMaxThreads>
 __global__ void __launch_bounds__(LPR ? kRowThreads : kMaxThreads)
 norm_bwd_regs(NormBwdArgs p) {
-  __shared__ __align__(512) float buf[128];
+  __shared__ __align__(1024) float buf[256];
   extern __shared__ __align__(16) float dyn[];   // kOdd: weight copies; then a warp row's sums
   float* red = buf;
   const int D = p.width;
@@ -393,7 +391,8 @@ norm_bwd_regs(NormBwdArgs p) {
     const size_t base = at.base(r, D);
     const float rstd = rstd_next, mean = mean_next;
     float xh[NV][8], g[NV][8];
-    float a = 0.f, b = 0.f;
+    float sums[2] = {0.f, 0.f};   // of g, of g xh
+    float &a = sums[0], &b = sums[1];
     if (dhp && live) {   // needed last: in flight over the reduction, not a row ahead
 #pragma unroll
       for (int v = 0; v < NV; ++v)
@@ -417,7 +416,7 @@ norm_bwd_regs(NormBwdArgs p) {
         }
       }
     fetch(r + at.step);
-    row_sums<LPR>(a, b, red);
+    row_sums<LPR>(sums, red);
     a = p.center ? a * inv : 0.f;
     b *= inv;
 #pragma unroll
@@ -471,7 +470,7 @@ norm_bwd_regs(NormBwdArgs p) {
 template <typename TS, typename TG, bool kDb>
 __global__ void __launch_bounds__(1024) norm_bwd_ring(NormBwdArgs p, int stages) {
   constexpr int NV = 2, US = sizeof(TS) / 2, UG = sizeof(TG) / 2;   // 16-byte units a group
-  __shared__ __align__(512) float buf[128];
+  __shared__ __align__(1024) float buf[256];
   extern __shared__ __align__(16) uint4 ring[];
   float* red = buf;
   const int tid = threadIdx.x, tpr = blockDim.x, D = p.width, groups = D / 8;
@@ -522,7 +521,8 @@ __global__ void __launch_bounds__(1024) norm_bwd_ring(NormBwdArgs p, int stages)
     else
       issue(r, 0);
     const float rstd = p.rstd[r], mean = p.center ? p.mean[r] : 0.f;
-    float a = 0.f, b = 0.f;
+    float sums[2] = {0.f, 0.f};   // of g, of g xh
+    float &a = sums[0], &b = sums[1];
     wait();
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(1024) norm_bwd_ring(NormBwdArgs p, int stages)
         }
       }
     }
-    row_sums<0>(a, b, red);
+    row_sums<0>(sums, red);
     a = p.center ? a * inv : 0.f;
     b *= inv;
 #pragma unroll
@@ -790,7 +790,8 @@ int row_grid(long long rows) {
 
 template <typename TX, typename TR, int NV, int LPR, bool kOdd>
 cudaError_t fwd_go(const NormFwdArgs& p, Shape sh, cudaStream_t st) {
-  auto k = norm_fwd_regs<TX, TR, NV, LPR, kOdd>;
+  constexpr int R = LPR == 0 && NV == 2 && !kOdd ? 2 : 1;
+  auto k = norm_fwd_regs<TX, TR, NV, LPR, kOdd, R>;
   const size_t copy = Place<NV, LPR, kOdd>::copy_floats(p.width) * sizeof(float) * slots_of(sh);
   const size_t smem = kOdd ? copy * ((p.weight ? 1 : 0) + (p.bias ? 1 : 0)) : 0;
   cudaError_t e = allow(k, smem);
