@@ -250,6 +250,10 @@ struct Rows {
   int64_t batch = 1, length = 1, stride_b = 0, stride_t = 0;
   bool from(const Tensor& t) {
     const int64_t n = t.dim() - 1;
+    if (t.numel() == 0) {
+      batch = length = 0;
+      return true;
+    }
     if (t.size(n) > 1 && t.stride(n) != 1) return false;
     batch = length = 1;
     stride_b = stride_t = 0;

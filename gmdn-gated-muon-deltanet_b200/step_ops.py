@@ -385,4 +385,7 @@ def mlp8(x: Tensor, w_up: Tensor, w_down: Tensor, w_gate: Optional[Tensor] = Non
     for w in (w_up, w_down, w_gate):
         if w is not None and w.dtype != x.dtype:
             raise TypeError(f"mlp8: x is {x.dtype}, a weight {w.dtype}")
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in (x, *weights)):
+        y, _ = act8_forward(F.linear(x, w_up), None if w_gate is None else F.linear(x, w_gate))
+        return F.linear(y, w_down)
     return _Mlp8Function.apply(x, w_up, w_down, w_gate)
