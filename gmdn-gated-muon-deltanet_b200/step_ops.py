@@ -337,6 +337,12 @@ class _Mlp8Function(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        # the products in the forward's type, whatever the caller's autocast asks for
+        with torch.autocast("cuda", enabled=False):
+            return _Mlp8Function.grads(ctx, dout)
+
+    @staticmethod
+    def grads(ctx, dout):
         w_up, w_down, w_gate, codes, scales, *more = ctx.saved_tensors
         gate = Packed8(*more[:2], ctx.dtype) if ctx.gated else None
         saved = Act8Saved(Packed8(codes, scales, ctx.dtype), gate)

@@ -725,6 +725,23 @@ def test_mlp8_autocast_and_kept_memory():
         pkg.mlp8(x, w1, w2)     # bf16 with fp32 weights outside autocast
 
 
+@pytest.mark.parametrize("gated", [False, True])
+def test_mlp8_backward_under_another_autocast(gated):
+    """An fp32 forward's backward inside an autocast region keeps fp32: equal bits."""
+    pkg = load_pkg()
+    g = _gen(13)
+    x = torch.randn(70, 64, generator=g).cuda().requires_grad_(True)
+    ws = [(torch.randn(s, generator=g) / 8).cuda().requires_grad_(True)
+          for s in ((130, 64), (64, 130), (130, 64))[:3 if gated else 2]]
+    dout = torch.randn(70, 64, generator=g).cuda()
+    want = torch.autograd.grad(pkg.mlp8(x, *ws), [x, *ws], dout)
+    out = pkg.mlp8(x, *ws)
+    with torch.autocast("cuda", dtype=BF):
+        got = torch.autograd.grad(out, [x, *ws], dout)
+    for a, b in zip(got, want):
+        assert a.dtype == FP and torch.equal(a, b)
+
+
 def _block(pkg, p, idx, targets):
     """Two residual branches and the head on the operators, as a model uses them."""
     h = p["emb"][idx]
