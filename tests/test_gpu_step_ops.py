@@ -655,6 +655,24 @@ def test_act8_tails():
             assert dgate is None or torch.isfinite(dgate).all()
 
 
+def test_act8_fp32_gelu_keeps_its_digits():
+    """The small side too: P(x) is a product t q e, relative to it the fit (2e-8), 11
+    roundings of which those of the sum's leading terms count in full (3.5e-7 in a model of
+    them), the exponential (2^-22) and the reciprocal (2^-23): 8e-7 and y's own rounding.
+    For |x| < 1 it is 1/2 + x R: two half ulps of at most 1 over P >= 0.158, 4e-7."""
+    pkg = load_pkg()
+    x = torch.cat([torch.linspace(-12, 12, 1 << 18), torch.linspace(-1.01, 1.01, 1 << 16),
+                   torch.tensor([1.0, -1.0, 14.0, 15.0, 16.0, 1e6, 1e-30, -1e-30])])
+    y, _ = pkg.act8_forward(x.cuda())
+    want = x.double() * torch.special.erfc(-x.double() / 2.0 ** 0.5) / 2
+    rel = ((y.cpu().double() - want) / want.abs().clamp_min(2.0 ** -126)).abs()
+    print("largest relative error", rel.max().item())
+    assert rel.max() <= 8e-7 + EPS
+    inf = float("inf")
+    bad, _ = pkg.act8_forward(torch.tensor([inf, -inf, float("nan"), 3.0]).cuda())
+    assert bad[0] == inf and bad[1].isnan() and bad[2].isnan()
+
+
 # ---------------------------------------------------------------------------
 # the MLP, and the operators together
 # ---------------------------------------------------------------------------
