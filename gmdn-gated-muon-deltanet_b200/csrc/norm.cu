@@ -21,14 +21,16 @@
 // with the 5 us join of the CTAs' column sums); 8192 x 4096 and wider fp32 rows
 // 0.87 to 0.92 both ways; 8192 x 8192 bf16 96 and 112 us (0.86, 0.73).
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
 #include <type_traits>
 
 #include "common.cuh"
-#include "cp_async.cuh"
 #include "step_ops.h"
+
+namespace cg = cooperative_groups;
 
 namespace gmdn {
 namespace {
@@ -53,6 +55,7 @@ namespace {
 constexpr int kSms = 148;
 constexpr int kRowThreads = 128; // CTA of warp rows
 constexpr int kMaxCta = 512;     // threads of a CTA row: 128 registers each
+constexpr int kPair = -2;        // LPR: a row lies over a cluster of two CTAs
 using bf16 = __nv_bfloat16;
 
 template <typename T>
@@ -108,7 +111,7 @@ __device__ __forceinline__ void store_group(void* base, size_t i, const float* v
 template <int LPR>
 __device__ __forceinline__ float lane_sum(float v) {
 #pragma unroll
-  for (int o = (LPR ? LPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  for (int o = (LPR > 0 ? LPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   return v;
 }
 template <int LPR, int N>
@@ -126,6 +129,31 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float*& red) {
     for (int i = 0; i < N; ++i) v[i] = warp_sum(lane < n ? red[32 * i + lane] : 0.f);
     red = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(red) ^ 512);
   }
+}
+// The same over the two CTAs of a row, in two steps: each warp writes its sums to both CTAs'
+// buffers and arrives at the cluster's barrier; then they wait and add.  The barrier's release
+// waits for a thread's outstanding accesses, so the next row is fetched between the steps
+// (2048 x 16384: 117 us against 141 with the loads before them).
+template <int N>
+__device__ __forceinline__ void pair_arrive(float (&v)[N], float* red) {
+  auto cluster = cg::this_cluster();
+  const int lane = threadIdx.x & 31, at = (threadIdx.x >> 5) + 16 * cluster.block_rank();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+  if (lane < 2) {
+    float* to = cluster.map_shared_rank(red, lane);
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[32 * i + at] = v[i];
+  }
+  cluster.barrier_arrive();
+}
+template <int N>
+__device__ __forceinline__ void pair_wait(float (&v)[N], float*& red) {
+  const int lane = threadIdx.x & 31, n = blockDim.x >> 5;
+  cg::this_cluster().barrier_wait();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = warp_sum(lane % 16 < n ? red[32 * i + lane] : 0.f);
+  red = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(red) ^ 512);
 }
 
 // 8 values rounded to bf16, in place, pairs at a time
@@ -149,17 +177,19 @@ struct None {};
 // Where a thread's part of its rows lies.
 template <int NV, int LPR, bool kOdd>
 struct Place {
-  static constexpr int kSlots = LPR ? kRowThreads / LPR : 1;   // rows a CTA has at a time
+  static constexpr bool kWarp = LPR > 0;
+  static constexpr int L = kWarp ? LPR : 1, kCtas = LPR == kPair ? 2 : 1;   // CTAs a row
+  static constexpr int kSlots = kWarp ? kRowThreads / L : 1;   // rows a CTA has at a time
   int tid, tpr, slot, lead, off, width;
   long long row, step;        // the thread's first row; `lead` more than its warp's first
   uint32_t mask[kOdd ? NV : 1];   // kOdd: the row's elements of each group
   __device__ __forceinline__ Place(int D) : width(D) {
-    tid = LPR ? threadIdx.x % (LPR ? LPR : 1) : threadIdx.x;
-    tpr = LPR ? LPR : blockDim.x;
-    slot = LPR ? threadIdx.x / (LPR ? LPR : 1) : 0;
-    lead = LPR ? slot % (32 / (LPR ? LPR : 32)) : 0;
-    row = static_cast<long long>(blockIdx.x) * kSlots + slot;
-    step = static_cast<long long>(gridDim.x) * kSlots;
+    tid = kWarp ? threadIdx.x % L : threadIdx.x + blockIdx.x % kCtas * blockDim.x;
+    tpr = kWarp ? L : kCtas * blockDim.x;
+    slot = kWarp ? threadIdx.x / L : 0;
+    lead = kWarp ? slot % (32 / (kWarp ? L : 32)) : 0;
+    row = static_cast<long long>(blockIdx.x / kCtas) * kSlots + slot;
+    step = static_cast<long long>(gridDim.x / kCtas) * kSlots;
     off = 0;
     if constexpr (kOdd) {
       off = static_cast<int>((row % 8 * (D % 8)) % 8);
@@ -194,7 +224,7 @@ struct Place {
   // a (width) parameter's shared copy for this thread's slot: column c at off + c, 0 around
   static __host__ __device__ int copy_floats(int D) { return (D + 14) / 8 * 8; }
   __device__ __forceinline__ void copy(float* dst, const float* src, int D) const {
-    for (int i = tid; i < copy_floats(D); i += tpr) {
+    for (int i = kWarp ? tid : threadIdx.x; i < copy_floats(D); i += kWarp ? tpr : blockDim.x) {
       const int c = i - off;
       dst[i] = c >= 0 && c < D ? src[c] : 0.f;
     }
@@ -216,7 +246,7 @@ struct Place {
 // rows with two groups a thread take two (8192 x 8192 bf16 layer norm: 96 us
 // against 109 one row a step, two CTAs an SM instead of one).
 template <typename TX, typename TR, int NV, int LPR, bool kOdd, int R>
-__global__ void __launch_bounds__(LPR ? kRowThreads : kMaxCta) norm_fwd_regs(NormFwdArgs p) {
+__global__ void __launch_bounds__(LPR > 0 ? kRowThreads : kMaxCta) norm_fwd_regs(NormFwdArgs p) {
   constexpr bool kRes = !std::is_same<TR, None>::value;
   using TL = typename std::conditional<kRes, TR, TX>::type;   // the residual's loads
   constexpr bool kHf32 = std::is_same<TX, float>::value || std::is_same<TR, float>::value;
@@ -345,7 +375,7 @@ __global__ void __launch_bounds__(LPR ? kRowThreads : kMaxCta) norm_fwd_regs(Nor
 // kMaxThreads: an odd width's masks do not fit the 128 registers of 512 threads; up to 256
 // they have 255.
 template <typename TS, typename TG, int NV, int LPR, bool kOdd, bool kDb, int kMaxThreads>
-__global__ void __launch_bounds__(LPR ? kRowThreads : kMaxThreads)
+__global__ void __launch_bounds__(LPR > 0 ? kRowThreads : kMaxThreads)
 norm_bwd_regs(NormBwdArgs p) {
   __shared__ __align__(1024) float buf[256];
   extern __shared__ __align__(16) float dyn[];   // kOdd: weight copies; then a warp row's sums
@@ -385,19 +415,23 @@ norm_bwd_regs(NormBwdArgs p) {
       dw[v][k] = 0.f;
       if constexpr (kDb) db[v][k] = 0.f;
     }
+  if constexpr (LPR == kPair) cg::this_cluster().sync();   // the other CTA's memory is there
   fetch(at.row);
   for (long long r = at.row; r - at.lead < p.rows; r += at.step) {
-    const bool live = LPR == 0 || LPR == 32 || r < p.rows;
+    const bool live = LPR <= 0 || LPR == 32 || r < p.rows;
     const size_t base = at.base(r, D);
     const float rstd = rstd_next, mean = mean_next;
     float xh[NV][8], g[NV][8];
     float sums[2] = {0.f, 0.f};   // of g, of g xh
     float &a = sums[0], &b = sums[1];
-    if (dhp && live) {   // needed last: in flight over the reduction, not a row ahead
+    auto fetch_dh = [&] {   // needed last: in flight over the reduction, not a row ahead
+      if (dhp && live) {
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
-        if (at.has(v)) at.load(rh[v], dhp, base + at.group(v) * 8, total);
-    }
+        for (int v = 0; v < NV; ++v)
+          if (at.has(v)) at.load(rh[v], dhp, base + at.group(v) * 8, total);
+      }
+    };
+    if constexpr (LPR != kPair) fetch_dh();
 #pragma unroll
     for (int v = 0; v < NV; ++v)
       if (at.has(v) && live) {
@@ -415,8 +449,15 @@ norm_bwd_regs(NormBwdArgs p) {
           b = fmaf(g[v][k], xh[v][k], b);
         }
       }
+    if constexpr (LPR == kPair) {
+      pair_arrive(sums, red);
+      fetch_dh();
+    }
     fetch(r + at.step);
-    row_sums<LPR>(sums, red);
+    if constexpr (LPR == kPair)
+      pair_wait(sums, red);
+    else
+      row_sums<LPR>(sums, red);
     a = p.center ? a * inv : 0.f;
     b *= inv;
 #pragma unroll
@@ -430,12 +471,12 @@ norm_bwd_regs(NormBwdArgs p) {
       }
   }
   if (!p.dw && !p.db) return;
-  float* out = p.partial + static_cast<size_t>(blockIdx.x) * 2 * D;
+  float* out = p.partial + static_cast<size_t>(blockIdx.x / at.kCtas) * 2 * D;
 #pragma unroll
   for (int which = 0; which < (kDb ? 2 : 1); ++which) {
     // CTA rows write the partial; warp rows their slot of `dyn` (over the weight copies)
-    float* dst = LPR ? dyn + at.slot * D : out + which * D;
-    if constexpr (LPR != 0) __syncthreads();
+    float* dst = LPR > 0 ? dyn + at.slot * D : out + which * D;
+    if constexpr (LPR > 0) __syncthreads();
 #pragma unroll
     for (int v = 0; v < NV; ++v)
       if (at.has(v)) {
@@ -446,7 +487,7 @@ norm_bwd_regs(NormBwdArgs p) {
           if (at.bits(v) >> k & 1) dst[at.group(v) * 8 - at.off + k] = t;
         }
       }
-    if constexpr (LPR != 0) {
+    if constexpr (LPR > 0) {
       __syncthreads();
       for (int c = threadIdx.x; c < D; c += kRowThreads) {
         float t = 0.f;
@@ -458,169 +499,60 @@ norm_bwd_regs(NormBwdArgs p) {
   }
 }
 
-// The backward of rows of 8200 to 16384 elements (multiples of 8), one CTA of up
-// to 1024 threads a row, two groups of 8 a thread.  A row's arrays do not fit
-// the 64 registers of so many threads, so what a thread needs of its next row
-// comes by cp.async into its own part of shared memory (two rows deep where
-// that fits) and is read there twice, before and after the row's sums; only dw
-// and db stay in registers.  2048 x 16384 (bf16, fp32 stream): 176 us against
-// 279 for rows read again from L2.  Up to 8192 elements rows in registers are
-// faster (8192 x 8192 bf16: 112 us against 152), since this way reads shared
-// memory and the weights twice.
-template <typename TS, typename TG, bool kDb>
-__global__ void __launch_bounds__(1024) norm_bwd_ring(NormBwdArgs p, int stages) {
-  constexpr int NV = 2, US = sizeof(TS) / 2, UG = sizeof(TG) / 2;   // 16-byte units a group
-  __shared__ __align__(1024) float buf[256];
-  extern __shared__ __align__(16) uint4 ring[];
-  float* red = buf;
-  const int tid = threadIdx.x, tpr = blockDim.x, D = p.width, groups = D / 8;
-  const float inv = 1.f / static_cast<float>(D);
-  const int units = NV * (US + UG + (p.dh ? US : 0));   // of a thread and stage
-  auto unit = [&](int stage, int i) { return ring + (stage * units + i) * tpr + tid; };
-  auto copy = [&](int stage, int at, const void* src, size_t bytes, int n) {
-    const char* q = static_cast<const char*>(src) + bytes;
-    for (int u = 0; u < n; ++u) cp_async_cg16(unit(stage, at + u), q + 16 * u);
-  };
-  auto issue = [&](long long row, int stage) {
-    if (row < p.rows) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int g = v * tpr + tid;
-        if (g < groups) {
-          const size_t i = static_cast<size_t>(row) * D + g * 8;
-          copy(stage, v * US, p.s, i * sizeof(TS), US);
-          copy(stage, NV * US + v * UG, p.dy, i * sizeof(TG), UG);
-          if (p.dh) copy(stage, NV * (US + UG) + v * US, p.dh, i * sizeof(TS), US);
-        }
-      }
-    }
-    cp_async_commit();
-  };
-  auto wait = [&] {   // for the current row: stages - 1 later ones may be on their way
-    if (stages == 1) cp_async_wait<0>();
-    else cp_async_wait<1>();
-  };
-  auto take = [&](auto& raw, int stage, int at) {
-    constexpr int n = sizeof(raw.r) / sizeof(uint4);
-#pragma unroll
-    for (int u = 0; u < n; ++u) raw.r[u] = *unit(stage, at + u);
-  };
-  float dw[NV][8], db[kDb ? NV : 1][8];
-#pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      dw[v][k] = 0.f;
-      if constexpr (kDb) db[v][k] = 0.f;
-    }
-  int stage = 0;
-  if (stages > 1) issue(blockIdx.x, 0);
-  for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    if (stages > 1)
-      issue(r + gridDim.x, stage ^ 1);
-    else
-      issue(r, 0);
-    const float rstd = p.rstd[r], mean = p.center ? p.mean[r] : 0.f;
-    float sums[2] = {0.f, 0.f};   // of g, of g xh
-    float &a = sums[0], &b = sums[1];
-    wait();
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = v * tpr + tid;
-      if (i < groups) {
-        Raw<TS> rs;
-        Raw<TG> rg;
-        take(rs, stage, v * US);
-        take(rg, stage, NV * US + v * UG);
-        float w[8];
-        if (p.weight) load_param8(p.weight + i * 8, w);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float xh = (rs.get(k) - mean) * rstd;
-          float g = rg.get(k);
-          dw[v][k] = fmaf(g, xh, dw[v][k]);
-          if constexpr (kDb) db[v][k] += g;
-          if (p.weight) g *= w[k];
-          a += g;
-          b = fmaf(g, xh, b);
-        }
-      }
-    }
-    row_sums<0>(sums, red);
-    a = p.center ? a * inv : 0.f;
-    b *= inv;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int i = v * tpr + tid;
-      if (i < groups) {
-        Raw<TS> rs, rh;
-        Raw<TG> rg;
-        take(rs, stage, v * US);
-        take(rg, stage, NV * US + v * UG);
-        if (p.dh) take(rh, stage, NV * (US + UG) + v * US);
-        float w[8], d[8];
-        if (p.weight) load_param8(p.weight + i * 8, w);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float xh = (rs.get(k) - mean) * rstd;
-          float g = rg.get(k);
-          if (p.weight) g *= w[k];
-          d[k] = fmaf(fmaf(xh, -b, g - a), rstd, p.dh ? rh.get(k) : 0.f);
-        }
-        const size_t at = static_cast<size_t>(r) * D + i * 8;
-        if (p.ds_a) store_group(p.ds_a, at, d, p.a_f32, 0xffu);
-        if (p.ds_b) store_group(p.ds_b, at, d, p.b_f32, 0xffu);
-      }
-    }
-    if (stages > 1) stage ^= 1;
-  }
-  cp_async_wait<0>();
-  if (!p.dw && !p.db) return;
-  float* out = p.partial + static_cast<size_t>(blockIdx.x) * 2 * D;
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int i = v * tpr + tid;
-    if (i < groups) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        out[i * 8 + k] = dw[v][k];
-        if constexpr (kDb) out[D + i * 8 + k] = db[v][k];
-      }
-    }
-  }
-}
-
 // How a width is held: by the most groups of 8 a row can touch.  Rows of up to
 // 96 groups by 8, 16 or 32 lanes (three groups a lane are as many as the
 // backward's five arrays of them leave registers for); CTA rows with two groups
-// a thread up to 1024 groups; up to 2048 the forward with four, the backward by
-// norm_bwd_ring.  Other wide rows are read again for each pass (lanes -1).
+// a thread up to 1024 groups; up to 2048 the forward with four (whose registers the
+// backward does not have), the backward by a cluster of two CTAs.  Two CTAs a row
+// pay for their barrier only where one cannot hold it: 2048 x 16384 (bf16, fp32
+// stream) backward 117 us, against 279 for rows read again from L2 and 68 us forward
+// (89 with two CTAs); 8192 x 8192 bf16 backward 111 us by one CTA, 171 by two.
+// Other wide rows are read again for each pass (nv 0).
 struct Shape {
-  int nv, lanes, threads;   // lanes 0: CTA rows
-  bool odd, ring;
+  int nv, lanes, threads;   // lanes 0: CTA rows, kPair: two CTAs a row
+  bool odd;
 };
 Shape shape_of(int D, bool fwd) {
   const bool odd = D % 8 != 0;
   const int groups = odd ? (D + 14) / 8 : D / 8;
   auto up = [&](int per) { return (groups + per * 32 - 1) / (per * 32) * 32; };
-  if (groups <= 8) return {1, 8, kRowThreads, odd, false};
-  if (groups <= 16) return {1, 16, kRowThreads, odd, false};
-  if (groups <= 96) return {(groups + 31) / 32, 32, kRowThreads, odd, false};
-  if (groups <= 2 * kMaxCta) return {2, 0, up(2), odd, false};
-  if (!fwd && !odd && groups <= 2048) return {2, 0, up(2), odd, true};
-  if (fwd && groups <= 4 * kMaxCta) return {4, 0, up(4), odd, false};
-  return {0, -1, 0, odd, false};
+  if (groups <= 8) return {1, 8, kRowThreads, odd};
+  if (groups <= 16) return {1, 16, kRowThreads, odd};
+  if (groups <= 96) return {(groups + 31) / 32, 32, kRowThreads, odd};
+  if (groups <= 2 * kMaxCta) return {2, 0, up(2), odd};
+  if (groups <= 4 * kMaxCta) return fwd ? Shape{4, 0, up(4), odd} : Shape{2, kPair, up(4), odd};
+  return {0, -1, 0, odd};
 }
+// A launch of clusters of two CTAs.
+struct ClusterLaunch {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  ClusterLaunch(int ctas, int threads, size_t smem, cudaStream_t st) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {2, 1, 1};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+};
 int slots_of(Shape sh) { return sh.lanes > 0 ? kRowThreads / sh.lanes : 1; }
 
-// One wave of CTAs, each walking rows a grid apart; for odd widths the step is a
-// multiple of 8 rows.
+// One wave of CTAs (kPair: of clusters, two CTAs each), each walking rows a grid apart;
+// for odd widths the step is a multiple of 8 rows.
 template <typename K>
 int wave(K kernel, long long rows, Shape sh, size_t smem) {
   const int slots = slots_of(sh);
   const long long want = (rows + slots - 1) / slots;
   long long grid = want;
-  if (want > kSms) {
+  if (sh.lanes == kPair) {
+    int n = 0;
+    ClusterLaunch at(2 * kSms, sh.threads, smem, nullptr);
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &at.cfg) != cudaSuccess || n < 8) n = 8;
+    if (n < grid) grid = n;
+  } else if (want > kSms) {
     int n = 1;
     cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, sh.threads, smem);
     const long long cap = static_cast<long long>(kSms) * (n < 1 ? 1 : n);
@@ -633,7 +565,6 @@ int wave(K kernel, long long rows, Shape sh, size_t smem) {
   return static_cast<int>(grid);
 }
 
-constexpr size_t kMaxRing = 220 * 1024;   // shared memory the stages may take
 template <typename K>
 cudaError_t allow(K kernel, size_t smem) {
   return smem <= 48 * 1024 ? cudaSuccess
@@ -816,35 +747,26 @@ cudaError_t fwd_typed(const NormFwdArgs& p, Shape sh, cudaStream_t st) {
   return sh.odd ? fwd_shaped<TX, TR, true>(p, sh, st) : fwd_shaped<TX, TR, false>(p, sh, st);
 }
 
-// Launches the rows' kernel with at most `most` CTAs; *parts: how many there are.
+// Launches the rows' kernel with at most `most` CTAs (kPair: clusters); *parts: how many there are.
 template <typename TS, typename TG, bool kDb, bool kOdd, int NV, int LPR, int kMaxThreads = kMaxCta>
 cudaError_t bwd_go(const NormBwdArgs& p, Shape sh, int most, int* parts, cudaStream_t st) {
   auto k = norm_bwd_regs<TS, TG, NV, LPR, kOdd, kDb, kMaxThreads>;
   const int slots = slots_of(sh);
   const size_t copies = kOdd && p.weight ? Place<NV, LPR, kOdd>::copy_floats(p.width) * slots : 0;
-  const size_t sums = LPR && (p.dw || p.db) ? static_cast<size_t>(p.width) * slots : 0;
+  const size_t sums = LPR > 0 && (p.dw || p.db) ? static_cast<size_t>(p.width) * slots : 0;
   const size_t smem = sizeof(float) * (copies > sums ? copies : sums);
   cudaError_t e = allow(k, smem);
   if (e != cudaSuccess) return e;
   int grid = wave(k, p.rows, sh, smem);
   if (grid > most) grid = most;   // a multiple of 8
   *parts = grid;
-  k<<<grid, sh.threads, smem, st>>>(p);
-  return cudaGetLastError();
-}
-template <typename TS, typename TG, bool kDb>
-cudaError_t bwd_ring(const NormBwdArgs& p, Shape sh, int most, int* parts, cudaStream_t st) {
-  auto k = norm_bwd_ring<TS, TG, kDb>;
-  const size_t row = static_cast<size_t>(sh.threads) * 16 *
-                     (sizeof(TS) * (p.dh ? 2 : 1) + sizeof(TG));
-  const int stages = 2 * row <= kMaxRing ? 2 : 1;
-  cudaError_t e = allow(k, row * stages);
-  if (e != cudaSuccess) return e;
-  int grid = wave(k, p.rows, sh, row * stages);
-  if (grid > most) grid = most;
-  *parts = grid;
-  k<<<grid, sh.threads, row * stages, st>>>(p, stages);
-  return cudaGetLastError();
+  if constexpr (LPR == kPair) {
+    ClusterLaunch at(2 * grid, sh.threads, smem, st);
+    return cudaLaunchKernelEx(&at.cfg, k, p);
+  } else {
+    k<<<grid, sh.threads, smem, st>>>(p);
+    return cudaGetLastError();
+  }
 }
 template <typename TS, typename TG, bool kDb, bool kOdd>
 cudaError_t bwd_shaped(const NormBwdArgs& p, Shape sh, int most, int* parts, cudaStream_t st) {
@@ -855,15 +777,13 @@ cudaError_t bwd_shaped(const NormBwdArgs& p, Shape sh, int most, int* parts, cud
     if (sh.nv == 2) return bwd_go<TS, TG, kDb, kOdd, 2, 32>(p, sh, most, parts, st);
     return bwd_go<TS, TG, kDb, kOdd, 3, 32>(p, sh, most, parts, st);
   }
+  if (sh.lanes == kPair) return bwd_go<TS, TG, kDb, kOdd, 2, kPair>(p, sh, most, parts, st);
   if (kOdd && sh.threads <= 256)
     return bwd_go<TS, TG, kDb, kOdd, 2, 0, 256>(p, sh, most, parts, st);
   return bwd_go<TS, TG, kDb, kOdd, 2, 0>(p, sh, most, parts, st);
 }
 template <typename TS, typename TG>
 cudaError_t bwd_typed(const NormBwdArgs& p, Shape sh, int most, int* parts, cudaStream_t st) {
-  if (sh.ring)
-    return p.db ? bwd_ring<TS, TG, true>(p, sh, most, parts, st)
-                : bwd_ring<TS, TG, false>(p, sh, most, parts, st);
   if (sh.odd)
     return p.db ? bwd_shaped<TS, TG, true, true>(p, sh, most, parts, st)
                 : bwd_shaped<TS, TG, false, true>(p, sh, most, parts, st);
@@ -875,7 +795,7 @@ cudaError_t bwd_typed(const NormBwdArgs& p, Shape sh, int most, int* parts, cuda
 
 cudaError_t norm_fwd(const NormFwdArgs& p, cudaStream_t st) {
   const Shape sh = shape_of(p.width, true);
-  if (sh.lanes < 0) {
+  if (sh.nv == 0) {
     norm_fwd_rows<<<row_grid(p.rows), kThreads, 0, st>>>(p);
     return cudaGetLastError();
   }
@@ -891,8 +811,8 @@ cudaError_t norm_fwd(const NormFwdArgs& p, cudaStream_t st) {
 // SM (an odd width's rounded to its grid's multiple of 8).
 int norm_bwd_partials(long long rows, int width) {
   const Shape sh = shape_of(width, false);
-  const int resident = sh.lanes < 0 ? 2 : sh.ring ? 1 : 512 / sh.threads;
-  const int all = kSms * (resident < 1 ? 1 : resident), cap = sh.odd ? all / 8 * 8 : all;
+  const int all = sh.nv == 0 ? 2 * kSms : sh.lanes == kPair ? kSms / 2 : kSms * (512 / sh.threads);
+  const int cap = sh.odd ? all / 8 * 8 : all;
   return static_cast<int>(rows < cap ? rows : cap);
 }
 
@@ -901,7 +821,7 @@ cudaError_t norm_bwd(const NormBwdArgs& p, cudaStream_t st) {
   const int most = norm_bwd_partials(p.rows, p.width);
   int parts = most;
   cudaError_t e;
-  if (sh.lanes >= 0) {
+  if (sh.nv > 0) {
     if (p.s_f32)
       e = p.dy_f32 ? bwd_typed<float, float>(p, sh, most, &parts, st)
                    : bwd_typed<float, bf16>(p, sh, most, &parts, st);

@@ -156,7 +156,8 @@ def test_norm_sizes(rows, D, center):
                                      (3001, 513), (2000, 761), (2500, 775), (2501, 1030),
                                      (1200, 4081), (1201, 4083), (700, 8177), (650, 8179),
                                      (300, 8191), (40, 16370), (3, 16383),
-                                     (300, 16384), (320, 8200)])
+                                     (300, 16384), (320, 8200), (301, 8185), (299, 8193),
+                                     (303, 12345), (200, 16377), (150, 16378)])
 def test_norm_ragged_widths(rows, D):
     """Rows at every alignment, each CTA walking many of them, at the borders
     between the ways a width is held."""
@@ -168,7 +169,7 @@ def test_norm_ragged_widths(rows, D):
 def test_norm_neighbours_stay_out():
     """Infinities and NaN in a row stay in it, whatever shares its memory groups."""
     pkg = load_pkg()
-    for D in (5, 100, 769, 1283):
+    for D in (5, 100, 769, 1283, 8203):
         c = _norm_case(24, D, True, FP, BF, FP)
         clean, cg = _run_norm(pkg, c)
         c["x"][7] = math.inf
