@@ -70,14 +70,31 @@ def _torch_dir() -> str:
     return spec.submodule_search_locations[0]
 
 
+def host_cxx() -> str:
+    """A host compiler that links the shared libstdc++, which torch's libraries use.  One that
+    has only libstdc++.a gives libgmdn_torch.so a second C++ runtime, and the first number
+    written into an error message then crashes the process."""
+    for cand in (os.environ.get("CXX"), "g++"):
+        path = cand and shutil.which(cand)
+        if not path:
+            continue
+        res = subprocess.run([path, "-print-file-name=libstdc++.so"], capture_output=True, text=True)
+        if res.returncode == 0 and os.path.isabs(res.stdout.strip()):
+            return path
+    raise RuntimeError("no C++ compiler with a shared libstdc++ ($CXX, g++): libgmdn_torch.so "
+                       "has to share torch's C++ runtime")
+
+
 def build_torch(force: bool = False) -> str:
     """libgmdn_torch.so: plain C++ (no device code), against the installed torch."""
     header = max(os.path.getmtime(h) for h in glob.glob(os.path.join(ROOT, "include", "*.h")))
+    # this file holds the flags
+    header = max(header, os.path.getmtime(os.path.abspath(__file__)))
     if not force and not _stale(TORCH_SRC, TORCH_LIB, header):
         return TORCH_LIB
     t = _torch_dir()
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+    cmd = [host_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared",
            "-D_GLIBCXX_USE_CXX11_ABI=1", "-I", os.path.join(t, "include"),
            "-I", os.path.join(t, "include", "torch", "csrc", "api", "include"),
            "-I", os.path.join(cuda, "include"), TORCH_SRC, "-o", TORCH_LIB + ".tmp",

@@ -1,0 +1,37 @@
+"""The step operators' own checks, below the Python ones: a refusal is an
+exception with its message.  The kernels' entries are reached through the
+dispatcher with CPU tensors; every call is refused before it touches a device.
+"""
+import pytest
+import torch
+
+from conftest import load_pkg
+
+CUDA = torch._C.DispatchKeySet(torch._C.DispatchKey.CUDA)
+
+
+def _op(name):
+    load_pkg()
+    return getattr(torch.ops.gmdn, name).default
+
+
+@pytest.mark.parametrize("name, args, error, message", [
+    ("norm_fwd", (torch.zeros(3, 8), None, torch.zeros(7), None, 1e-5, True, True), RuntimeError,
+     "expected 8 float32 values"),
+    ("norm_fwd", (torch.zeros(3, 8).half(), None, None, None, 1e-5, True, True), TypeError,
+     "must be bfloat16 or float32, got Half"),
+    ("norm_fwd", (torch.zeros(3, 8), torch.zeros(2, 8), None, None, 1e-5, True, True),
+     RuntimeError, "differ in shape"),
+    ("norm_fwd", (torch.zeros(3, 8), torch.zeros(3, 8, device="meta"), None, None, 1e-5, True,
+                  True), RuntimeError, "tensors on cpu and meta"),
+    ("norm_bwd", (torch.zeros(3, 8), torch.zeros(2, 4), None, torch.zeros(3, 8), None, True, False,
+                  True, False, False), RuntimeError, "expected 6 float32 values"),
+    ("token_logprobs_fwd", (torch.zeros(3, 0), None, True, 0, -100), RuntimeError, "logits must be"),
+    ("token_logprobs_bwd", (torch.zeros(3, 9), None, None, torch.zeros(3, 3), None, None, None,
+                            -100), RuntimeError, "expected 12 float32 values"),
+    ("unpack8", (torch.zeros(300, dtype=torch.int8), torch.zeros(2), True), ValueError,
+     "one scale for each 128"),
+])
+def test_a_refusal_is_an_exception(name, args, error, message):
+    with pytest.raises(error, match=message):
+        _op(name).redispatch(CUDA, *args)
