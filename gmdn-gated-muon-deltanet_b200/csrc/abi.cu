@@ -437,12 +437,15 @@ int gmdn_norm_bwd(const void* s, const float* rstd, const float* mean, const flo
   if (!s || !rstd || !dy || (center && !mean)) return fail(GMDN_ERR_INVALID, "norm: null pointer");
   if (misaligned({s, weight, dy, dh, ds_a, ds_b}))
     return fail(GMDN_ERR_INVALID, "norm: pointers must be 16-byte aligned");
+  // dh is the cotangent of h, which is s: the kernels read it as such
+  if (dh && (dh_f32 != 0) != (s_f32 != 0))
+    return fail(GMDN_ERR_INVALID, "norm: dh must have the type of s");
   const size_t need = gmdn_norm_bwd_workspace_bytes(rows, width);
   if ((dweight || dbias) && (!workspace || workspace_bytes < need))
     return fail(GMDN_ERR_WORKSPACE, "workspace %zu bytes < required %zu", workspace_bytes, need);
   gmdn::NormBwdArgs p{s, rstd, mean, weight, dy, dh, ds_a, ds_b, dweight, dbias,
                       static_cast<float*>(workspace), rows, width, center != 0, s_f32 != 0,
-                      dy_f32 != 0, dh_f32 != 0, a_f32 != 0, b_f32 != 0};
+                      dy_f32 != 0, a_f32 != 0, b_f32 != 0};
   GMDN_LAUNCH(gmdn::norm_bwd(p, st), "norm_bwd");
   return GMDN_OK;
 }

@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kThreads) norm_bwd_rows(NormBwdArgs p) {
       float g = load_act(p.dy, base + i, p.dy_f32);
       if (p.weight) g *= p.weight[i];
       float d = (g - a - xh * b) * rstd;
-      if (p.dh) d += load_act(p.dh, base + i, p.dh_f32);
+      if (p.dh) d += load_act(p.dh, base + i, p.s_f32);
       if (p.ds_a) store_act(p.ds_a, base + i, d, p.a_f32);
       if (p.ds_b) store_act(p.ds_b, base + i, d, p.b_f32);
     }

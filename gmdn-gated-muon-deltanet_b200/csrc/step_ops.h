@@ -21,13 +21,13 @@ struct NormFwdArgs {
 struct NormBwdArgs {
   const void* s;                 // what was normalised: x, or h
   const float *rstd, *mean, *weight;
-  const void *dy, *dh;           // dh may be null
+  const void *dy, *dh;           // dh: in the type of s, may be null
   void *ds_a, *ds_b;             // the gradient of s in one or two types (either may be null)
   float *dw, *db;                // either may be null
   float* partial;                // norm_bwd_partials(...) x 2 x width floats
   long long rows;
   int width;
-  bool center, s_f32, dy_f32, dh_f32, a_f32, b_f32;
+  bool center, s_f32, dy_f32, a_f32, b_f32;
 };
 cudaError_t norm_fwd(const NormFwdArgs& p, cudaStream_t st);
 int norm_bwd_partials(long long rows, int width);

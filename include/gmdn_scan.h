@@ -245,7 +245,8 @@ int gmdn_norm_fwd(const void* x, const void* residual, const float* weight, cons
 size_t gmdn_norm_bwd_workspace_bytes(long long rows, int width);
 
 /* Backward: s is what was normalised (x, or h), dy the cotangent of y, dh that
- * of h (NULL: none).  The gradient of s (dh included) is written to ds_a and
+ * of h (NULL: none), of the type of s: dh_f32 has to equal s_f32.  The
+ * gradient of s (dh included) is written to ds_a and
  * ds_b in the type of each (either may be NULL: x and residual share it).
  * dweight, dbias (width, fp32; either may be NULL) are overwritten; they are
  * summed in a fixed order, so equal calls give equal bits. */

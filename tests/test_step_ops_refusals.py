@@ -2,11 +2,15 @@
 exception with its message.  The kernels' entries are reached through the
 dispatcher with CPU tensors; every call is refused before it touches a device.
 """
+import ctypes
+
 import pytest
 import torch
 
 from conftest import load_pkg
 
+NULL = ctypes.c_void_p(None)
+FAKE = ctypes.c_void_p(0x1000)   # never dereferenced: the checks fail first
 CUDA = torch._C.DispatchKeySet(torch._C.DispatchKey.CUDA)
 
 
@@ -35,3 +39,20 @@ def _op(name):
 def test_a_refusal_is_an_exception(name, args, error, message):
     with pytest.raises(error, match=message):
         _op(name).redispatch(CUDA, *args)
+
+
+@pytest.mark.parametrize("width", [64, 768, 1283, 8192, 16384, 40000])
+@pytest.mark.parametrize("s_f32", [0, 1])
+def test_norm_abi_refuses_a_dh_of_another_type(width, s_f32):
+    """The kernels read dh as h is stored: another type would be read past its end."""
+    lib = load_pkg()._lib.lib
+
+    def bwd(dh, dh_f32):
+        return lib.gmdn_norm_bwd(FAKE, FAKE, FAKE, FAKE, FAKE, dh, FAKE, NULL, NULL, NULL, NULL, 0,
+                                 -1 if dh_f32 == s_f32 or not dh.value else 100, width, 1, s_f32, 0,
+                                 dh_f32, 0, 0, NULL)
+
+    assert bwd(FAKE, 1 - s_f32) == 1
+    assert "type of s" in lib.gmdn_last_error_string().decode()
+    assert bwd(FAKE, s_f32) == 1 and bwd(NULL, 1 - s_f32) == 1   # refused for their size alone
+    assert "negative size" in lib.gmdn_last_error_string().decode()
