@@ -56,6 +56,7 @@ constexpr int kSms = 148;
 constexpr int kRowThreads = 128; // CTA of warp rows
 constexpr int kMaxCta = 512;     // threads of a CTA row: 128 registers each
 constexpr int kPair = -2;        // LPR: a row lies over a cluster of two CTAs
+constexpr int kBuf = 256;        // floats a CTA's sums go through: two buffers of 128
 using bf16 = __nv_bfloat16;
 
 template <typename T>
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(LPR > 0 ? kRowThreads : kMaxCta) norm_fwd_regs
   constexpr bool kRes = !std::is_same<TR, None>::value;
   using TL = typename std::conditional<kRes, TR, TX>::type;   // the residual's loads
   constexpr bool kHf32 = std::is_same<TX, float>::value || std::is_same<TR, float>::value;
-  __shared__ __align__(1024) float buf[256];
+  __shared__ __align__(1024) float buf[kBuf];
   extern __shared__ __align__(16) float params[];   // kOdd: weight, bias, a copy a slot
   float* red = buf;
   const int D = p.width;
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(LPR > 0 ? kRowThreads : kMaxCta) norm_fwd_regs
 template <typename TS, typename TG, int NV, int LPR, bool kOdd, bool kDb, int kMaxThreads>
 __global__ void __launch_bounds__(LPR > 0 ? kRowThreads : kMaxThreads)
 norm_bwd_regs(NormBwdArgs p) {
-  __shared__ __align__(1024) float buf[256];
+  __shared__ __align__(1024) float buf[kBuf];
   extern __shared__ __align__(16) float dyn[];   // kOdd: weight copies; then a warp row's sums
   float* red = buf;
   const int D = p.width;
@@ -565,11 +566,13 @@ int wave(K kernel, long long rows, Shape sh, size_t smem) {
   return static_cast<int>(grid);
 }
 
+// 48 KB, the kernel's own `buf` counted, is what a launch may use without being asked for more.
 template <typename K>
 cudaError_t allow(K kernel, size_t smem) {
-  return smem <= 48 * 1024 ? cudaSuccess
-                           : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                  static_cast<int>(smem));
+  return smem + kBuf * sizeof(float) <= 48 * 1024
+             ? cudaSuccess
+             : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    static_cast<int>(smem));
 }
 
 // ---------------------------------------------------------------------------
