@@ -631,7 +631,8 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
     const int64_t tt = p.targets[r];
     if (tt != p.ignore_index) {
       const bool ok = tt >= 0 && tt < V;
-      gl = ok ? p.g_logprobs[r] : nan;
+      gl = p.g_logprobs[r];
+      if (!ok && gl != 0.f) gl = nan;
       t = ok ? static_cast<int>(tt) : -1;
     }
   }
