@@ -71,22 +71,29 @@ void check_f32(const char* op, const OptTensor& t, int64_t n) {
   TORCH_CHECK(!has(t) || (is_f32(*t) && t->numel() == n), op, ": expected ", n,
               " float32 values");
 }
-// Whether autograd has anything to record.
-bool any_requires_grad(std::initializer_list<const Tensor*> ts,
-                       std::initializer_list<const OptTensor*> opts) {
-  if (!c10::GradMode::is_enabled()) return false;
+// A forward-mode tangent: it needs neither requires_grad nor grad mode.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+// Whether autograd has anything to record, or a tangent to refuse (there is no forward mode, and
+// autograd's path says so).
+bool any_derivative(std::initializer_list<const Tensor*> ts,
+                    std::initializer_list<const OptTensor*> opts) {
+  const bool grad = c10::GradMode::is_enabled();
+  auto wants = [grad](const Tensor& t) { return (grad && t.requires_grad()) || has_tangent(t); };
   for (const Tensor* t : ts)
-    if (t->requires_grad()) return true;
+    if (wants(*t)) return true;
   for (const OptTensor* t : opts)
-    if (has(*t) && (*t)->requires_grad()) return true;
+    if (has(*t) && wants(**t)) return true;
   return false;
 }
-// In a plain backward (grad mode off) its op goes straight to the kernel, past the boxed
-// fallback that refuses second derivatives.
+// In a plain backward (grad mode off, cotangents without tangents) its op goes straight to the
+// kernel, past the boxed fallback that refuses second derivatives and tangents.
 struct BelowAutograd {
   std::optional<at::AutoDispatchBelowADInplaceOrView> guard;
-  BelowAutograd() {
-    if (!c10::GradMode::is_enabled()) guard.emplace();
+  explicit BelowAutograd(const variable_list& cotangents) {
+    if (c10::GradMode::is_enabled()) return;
+    for (const Tensor& t : cotangents)
+      if (has_tangent(t)) return;
+    guard.emplace();
   }
 };
 void* stream_of(const Tensor& t) {
@@ -216,7 +223,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
                                          : at::zeros_like(s, s.options().dtype(dy_type));
     const OptTensor dh = res && grads[1].defined() ? OptTensor(grads[1]) : OptTensor();
     const bool need_x = flag(kNeedX), need_res = flag(kNeedRes);
-    const BelowAutograd below;
+    const BelowAutograd below(grads);
     auto [da, db, dw, dbias] =
         norm_bwd_op(s, saved[1], w.defined() ? OptTensor(w) : OptTensor(), dy, dh, flag(kCenter),
                     (need_x && !x_f32) || (need_res && !res_f32),
@@ -229,7 +236,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
 
 Norm norm_fwd_autograd(const Tensor& x, const OptTensor& res, const OptTensor& w,
                        const OptTensor& b, double eps, bool center, bool out_f32) {
-  if (!any_requires_grad({&x}, {&res, &w, &b})) {
+  if (!any_derivative({&x}, {&res, &w, &b})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return norm_fwd_op(x, res, w, b, eps, center, out_f32);
   }
@@ -400,7 +407,7 @@ struct LogprobsFunction : torch::autograd::Function<LogprobsFunction> {
     auto cot = [&](int i, bool used) {
       return used && grads[i].defined() ? OptTensor(grads[i].to(at::kFloat)) : OptTensor();
     };
-    const BelowAutograd below;
+    const BelowAutograd below(grads);
     Tensor g = token_logprobs_bwd_op(
         saved[0], opt(saved[1]), opt(saved[2]), saved[3], cot(0, saved[1].defined()),
         cot(1, ctx->saved_data["entropy"].toBool()), cot(2, ctx->saved_data["top_k"].toInt() > 0),
@@ -411,7 +418,7 @@ struct LogprobsFunction : torch::autograd::Function<LogprobsFunction> {
 
 Logprobs token_logprobs_fwd_autograd(const Tensor& logits, const OptTensor& targets, bool entropy,
                                      int64_t top_k, int64_t ignore_index) {
-  if (!any_requires_grad({&logits}, {})) {
+  if (!any_derivative({&logits}, {})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return token_logprobs_fwd_op(logits, targets, entropy, top_k, ignore_index);
   }

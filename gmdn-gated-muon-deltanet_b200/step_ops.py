@@ -15,7 +15,9 @@
     tensor; a GELU or SwiGLU whose backward reads the checkpoint; and an MLP
     whose saved activations are all 8-bit (train_ablation.py:202-205).
 
-All run only on CUDA tensors, bf16 or fp32, through ``libgmdn_b200.so``.  The
+Derivatives are of the first order and reverse mode; second ones, and forward
+mode, raise.  All run only on CUDA tensors, bf16 or fp32, through
+``libgmdn_b200.so``.  The
 operators below them are registered in C++ (``csrc/torch_ops.cpp``) with their
 autograd formulas; here are their fake kernels (for torch.compile), the
 arguments' checks and the public names.
@@ -28,6 +30,7 @@ from typing import NamedTuple, Optional
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from ._lib import load_torch_ops
@@ -284,7 +287,8 @@ def unpack8(packed: Packed8) -> Tensor:
 def act8_forward(x: Tensor, gate: Optional[Tensor] = None) -> tuple[Tensor, Act8Saved]:
     """GELU(x) (exact), or SiLU(gate) * x with a gate, and the 8-bit checkpoint
     of its inputs for ``act8_backward``.  x, gate: one shape and type, bf16 or
-    fp32.  Not recorded by autograd (``mlp8`` is the differentiable form)."""
+    fp32.  Not seen by autograd, in reverse or forward mode (``mlp8`` is the
+    differentiable form)."""
     _f32_flag(x, "x")
     if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
         raise ValueError(f"gate must be like x, {tuple(x.shape)} {x.dtype}, got "
@@ -316,6 +320,11 @@ def act8_backward(saved: Act8Saved, dy: Tensor, restore: bool = True):
     return dx, dgate if gate is not None else None, y if restore else None
 
 
+def _has_tangent(*tensors: Optional[Tensor]) -> bool:
+    """A forward-mode tangent on any of them (it needs no requires_grad)."""
+    return any(t is not None and unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _Mlp8Function(torch.autograd.Function):
     """down(act(up x)) that keeps x and the activation's inputs in 8 bits; the
     weight gradients are products with the restored tensors."""
@@ -337,6 +346,8 @@ class _Mlp8Function(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        if _has_tangent(dout):
+            raise RuntimeError("mlp8: no forward-mode derivative of its backward")
         # the products in the forward's type, whatever the caller's autocast asks for
         with torch.autocast("cuda", enabled=False):
             return _Mlp8Function.grads(ctx, dout)
@@ -391,7 +402,9 @@ def mlp8(x: Tensor, w_up: Tensor, w_down: Tensor, w_gate: Optional[Tensor] = Non
     for w in (w_up, w_down, w_gate):
         if w is not None and w.dtype != x.dtype:
             raise TypeError(f"mlp8: x is {x.dtype}, a weight {w.dtype}")
-    if not torch.is_grad_enabled() or not any(t.requires_grad for t in (x, *weights)):
+    recorded = torch.is_grad_enabled() and any(t.requires_grad for t in (x, *weights))
+    # a tangent goes to autograd too, which refuses it
+    if not recorded and not _has_tangent(x, *weights):
         y, _ = act8_forward(F.linear(x, w_up), None if w_gate is None else F.linear(x, w_gate))
         return F.linear(y, w_down)
     return _Mlp8Function.apply(x, w_up, w_down, w_gate)

@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from conftest import load_pkg
 from oracle import step_oracle as so
@@ -46,3 +47,34 @@ def test_logprobs_bad_targets_without_cotangents_have_no_gradient(dtype):
     ent = pkg.token_logprobs(z, None, entropy=True).entropy
     (want,) = torch.autograd.grad(ent, z, b)
     assert torch.equal(g, want)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_mlp8_refuses_forward_mode(gated):
+    pkg = load_pkg()
+    g = _gen(3)
+    ps = [torch.randn(s, generator=g).cuda() for s in ((3, 64), (128, 64), (64, 128), (128, 64))]
+    ps = ps[:4 if gated else 3]
+    for grad in (False, True):
+        for i, p in enumerate(ps):
+            with torch.set_grad_enabled(grad), fw.dual_level(), \
+                    pytest.raises((RuntimeError, NotImplementedError)):
+                pkg.mlp8(*ps[:i], fw.make_dual(p, torch.ones_like(p)), *ps[i + 1:])
+            with torch.set_grad_enabled(grad), pytest.raises((RuntimeError, NotImplementedError)):
+                torch.func.jvp(lambda d: pkg.mlp8(*ps[:i], d, *ps[i + 1:]), (p,), (p,))
+    x = ps[0].clone().requires_grad_(True)
+    out = pkg.mlp8(x, *ps[1:])
+    with fw.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        torch.autograd.grad(out, x, fw.make_dual(torch.ones_like(out), torch.ones_like(out)))
+    with fw.dual_level():       # no tangent among the inputs: nothing to refuse
+        plain = pkg.mlp8(x.detach(), *ps[1:])
+    assert torch.equal(plain, out)
+
+
+def test_mlp8_without_gradients_compiles_whole():
+    pkg = load_pkg()
+    torch._dynamo.reset()
+    g = _gen(4)
+    ps = [torch.randn(s, generator=g).cuda() for s in ((40, 64), (128, 64), (64, 128))]
+    got = torch.compile(lambda *p: pkg.mlp8(*p), fullgraph=True, dynamic=False)(*ps)
+    assert torch.allclose(got, pkg.mlp8(*ps), rtol=1e-5, atol=1e-4)
