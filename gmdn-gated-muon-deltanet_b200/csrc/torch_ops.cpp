@@ -218,11 +218,21 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     auto flag = [flags](int64_t f) { return (flags & f) != 0; };
     const Tensor &s = saved[0], &w = saved[2];
     const bool res = flag(kRes), x_f32 = flag(kXF32), res_f32 = flag(kResF32);
-    const auto dy_type = flag(kOutF32) ? at::kFloat : at::kBFloat16;
-    const Tensor dy = grads[0].defined() ? grads[0].to(dy_type)
-                                         : at::zeros_like(s, s.options().dtype(dy_type));
     const OptTensor dh = res && grads[1].defined() ? OptTensor(grads[1]) : OptTensor();
     const bool need_x = flag(kNeedX), need_res = flag(kNeedRes);
+    if (!grads[0].defined()) {
+      // y is not used: the cotangent of h alone (the formula would make NaN of 0 times a row
+      // that holds an infinity)
+      auto as = [&](bool need, bool f32) {
+        return need && has(dh) ? dh->to(f32 ? at::kFloat : at::kBFloat16) : Tensor();
+      };
+      auto none = [&](int64_t f) {
+        return flag(f) ? at::zeros({s.size(-1)}, f32_like(s)) : Tensor();
+      };
+      return {as(need_x, x_f32), as(need_res, res_f32), none(kNeedW), none(kNeedB),
+              Tensor(), Tensor(), Tensor()};
+    }
+    const Tensor dy = grads[0].to(flag(kOutF32) ? at::kFloat : at::kBFloat16);
     const BelowAutograd below(grads);
     auto [da, db, dw, dbias] =
         norm_bwd_op(s, saved[1], w.defined() ? OptTensor(w) : OptTensor(), dy, dh, flag(kCenter),

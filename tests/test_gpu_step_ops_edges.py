@@ -78,3 +78,23 @@ def test_mlp8_without_gradients_compiles_whole():
     ps = [torch.randn(s, generator=g).cuda() for s in ((40, 64), (128, 64), (64, 128))]
     got = torch.compile(lambda *p: pkg.mlp8(*p), fullgraph=True, dynamic=False)(*ps)
     assert torch.allclose(got, pkg.mlp8(*ps), rtol=1e-5, atol=1e-4)
+
+
+@pytest.mark.parametrize("x_dt, res_dt", [(BF, FP), (FP, BF), (BF, BF), (FP, FP)])
+@pytest.mark.parametrize("D", [64, 1283, 16384])
+def test_norm_with_only_h_used(x_dt, res_dt, D):
+    """Without a cotangent of y the gradient is that of h, whatever the rows hold."""
+    pkg = load_pkg()
+    c = _norm_case(4, D, True, x_dt, res_dt, BF)
+    c["x"][1, 5 % D] = math.inf
+    c["x"][2, 3 % D] = math.nan
+    leaves = [c[n].cuda().requires_grad_(True) for n in ("x", "res", "w", "b")]
+    for call in (pkg.layer_norm, pkg.rms_norm):
+        _, h = call(leaves[0], leaves[2], leaves[3], 1e-5, residual=leaves[1])
+        dh = c["dh"].cuda()
+        dx, dr, dw, db = torch.autograd.grad(h, leaves, dh)
+        assert torch.equal(dx, dh.to(x_dt)) and torch.equal(dr, dh.to(res_dt))
+        assert not dw.any() and not db.any() and dw.shape == db.shape == (D,)
+        (dx,) = torch.autograd.grad(
+            call(leaves[0], residual=leaves[1].detach())[1], leaves[0], dh)
+        assert torch.equal(dx, dh.to(x_dt))
