@@ -12,6 +12,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libgmdn_b200.so")
 TORCH_LIB_PATH = os.path.join(_HERE, "libgmdn_torch.so")
+TORCH_STAMP = os.path.join(_HERE, "_build", "libgmdn_torch.torch_version")   # build.py writes it
 
 GMDN_PREC_IEEE = 0
 GMDN_PREC_FAST = 1
@@ -111,13 +112,22 @@ lib.gmdn_act8_bwd.argtypes = [_p] * 8 + [_q, _i, _p]
 
 
 def load_torch_ops() -> None:
-    """Register the operators of ``libgmdn_torch.so`` (torch.ops.gmdn.*)."""
+    """Register the operators of ``libgmdn_torch.so`` (torch.ops.gmdn.*).  ImportError where it
+    is missing, was built against another torch, or does not load."""
     import torch
+    build = f"build it with `python {os.path.join(_HERE, 'build.py')}`"
     if not os.path.exists(TORCH_LIB_PATH):
-        raise ImportError(
-            f"{TORCH_LIB_PATH} is missing: build it with "
-            f"`python {os.path.join(_HERE, 'build.py')}`")
-    torch.ops.load_library(TORCH_LIB_PATH)
+        raise ImportError(f"{TORCH_LIB_PATH} is missing: {build}")
+    if os.path.exists(TORCH_STAMP):
+        with open(TORCH_STAMP) as f:
+            version = f.read().strip()
+        if version != torch.__version__:
+            raise ImportError(f"{TORCH_LIB_PATH} was built against torch {version}, this is "
+                              f"{torch.__version__}: {build}")
+    try:
+        torch.ops.load_library(TORCH_LIB_PATH)
+    except OSError as e:
+        raise ImportError(f"{TORCH_LIB_PATH} does not load ({e}): {build}") from e
 
 
 def check(rc: int, what: str) -> None:

@@ -7,7 +7,8 @@ Every ``csrc/*.cu`` file is compiled by nvcc for ``sm_100a`` only
 ``libgmdn_b200.so`` next to this file.  The library exposes the C ABI of
 ``include/gmdn_scan.h`` and nothing else; it does not depend on torch.
 ``csrc/torch_ops.cpp`` (torch operators over that ABI) becomes
-``libgmdn_torch.so``, which links it and the installed torch.
+``libgmdn_torch.so``, which links it and the installed torch; it is built again
+for another torch, and left out where there is none.
 A file is recompiled only when it or any header it may include is newer than
 its object, so repeated calls are cheap.
 """
@@ -19,6 +20,7 @@ import concurrent.futures as cf
 import glob
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -30,6 +32,7 @@ BUILD = os.path.join(PKG_DIR, "_build")
 LIB = os.path.join(PKG_DIR, "libgmdn_b200.so")
 TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
 TORCH_LIB = os.path.join(PKG_DIR, "libgmdn_torch.so")
+TORCH_STAMP = os.path.join(BUILD, "libgmdn_torch.torch_version")   # what it was built against
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-Xptxas", "-warn-spills"]
@@ -63,11 +66,25 @@ def _compile(src: str, obj: str, extra: list[str]) -> tuple[str, str]:
     return src, res.stderr
 
 
-def _torch_dir() -> str:
+def _torch_dir() -> str | None:
     spec = importlib.util.find_spec("torch")
-    if spec is None:
-        raise RuntimeError("torch not found: libgmdn_torch.so is built against it")
-    return spec.submodule_search_locations[0]
+    return spec.submodule_search_locations[0] if spec else None
+
+
+def _torch_version(torch_dir: str) -> str:
+    """torch.__version__ without the import."""
+    with open(os.path.join(torch_dir, "version.py")) as f:
+        return re.search(r"^__version__\s*=\s*['\"](.+)['\"]", f.read(), re.M).group(1)
+
+
+def _torch_stale(version: str) -> bool:
+    # this file holds the flags
+    newest = max(os.path.getmtime(p) for p in [
+        os.path.abspath(__file__), *glob.glob(os.path.join(ROOT, "include", "*.h"))])
+    if _stale(TORCH_SRC, TORCH_LIB, newest) or not os.path.exists(TORCH_STAMP):
+        return True
+    with open(TORCH_STAMP) as f:
+        return f.read().strip() != version
 
 
 def host_cxx() -> str:
@@ -85,14 +102,17 @@ def host_cxx() -> str:
                        "has to share torch's C++ runtime")
 
 
-def build_torch(force: bool = False) -> str:
-    """libgmdn_torch.so: plain C++ (no device code), against the installed torch."""
-    header = max(os.path.getmtime(h) for h in glob.glob(os.path.join(ROOT, "include", "*.h")))
-    # this file holds the flags
-    header = max(header, os.path.getmtime(os.path.abspath(__file__)))
-    if not force and not _stale(TORCH_SRC, TORCH_LIB, header):
-        return TORCH_LIB
+def build_torch(force: bool = False) -> str | None:
+    """libgmdn_torch.so: plain C++ (no device code), against the installed torch; None without
+    one."""
     t = _torch_dir()
+    if t is None:
+        print("torch not found: libgmdn_torch.so is not built (libgmdn_b200.so does not need it)",
+              file=sys.stderr)
+        return None
+    version = _torch_version(t)
+    if not force and not _torch_stale(version):
+        return TORCH_LIB
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
     cmd = [host_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared",
            "-D_GLIBCXX_USE_CXX11_ABI=1", "-I", os.path.join(t, "include"),
@@ -104,6 +124,9 @@ def build_torch(force: bool = False) -> str:
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {os.path.basename(TORCH_SRC)}:\n{res.stdout}\n{res.stderr}")
     os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    os.makedirs(BUILD, exist_ok=True)
+    with open(TORCH_STAMP, "w") as f:
+        f.write(version)
     return TORCH_LIB
 
 

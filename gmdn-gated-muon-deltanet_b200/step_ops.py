@@ -39,12 +39,32 @@ from .ops import _f32_flag, _require_cuda
 __all__ = ["layer_norm", "rms_norm", "token_logprobs", "TokenLogprobs", "pack8", "unpack8",
            "Packed8", "act8_forward", "act8_backward", "Act8Saved", "mlp8"]
 
-load_torch_ops()
-_ops = torch.ops.gmdn
-_norm_fwd = _ops.norm_fwd.default
-_token_logprobs_fwd = _ops.token_logprobs_fwd.default
-_pack8, _unpack8 = _ops.pack8.default, _ops.unpack8.default
-_act8_fwd, _act8_bwd = _ops.act8_fwd.default, _ops.act8_bwd.default
+# The mixer's ops need libgmdn_b200.so alone: without libgmdn_torch.so the package still imports,
+# and the calls of this module raise why.
+try:
+    load_torch_ops()
+    _unloaded = None
+except ImportError as e:
+    _unloaded = str(e)
+
+
+def _op(name: str):
+    if _unloaded is None:
+        return getattr(torch.ops.gmdn, name).default
+
+    def missing(*_args):
+        raise ImportError(_unloaded)
+    return missing
+
+
+def _register_fake(name: str):
+    return torch.library.register_fake(f"gmdn::{name}") if _unloaded is None else lambda f: f
+
+
+_norm_fwd = _op("norm_fwd")
+_token_logprobs_fwd = _op("token_logprobs_fwd")
+_pack8, _unpack8 = _op("pack8"), _op("unpack8")
+_act8_fwd, _act8_bwd = _op("act8_fwd"), _op("act8_bwd")
 MAX_TOP_K = 64
 BLOCK8 = 128   # consecutive elements that share a scale
 
@@ -64,7 +84,7 @@ def _same_device(name: str, first: Tensor, *others: Optional[Tensor]) -> None:
 # norm over the model width
 # ---------------------------------------------------------------------------
 
-@torch.library.register_fake("gmdn::norm_fwd")
+@_register_fake("norm_fwd")
 def _(x, residual, weight, bias, eps, center, out_f32):
     D = x.shape[-1]
     y = x.new_empty(x.shape, dtype=torch.float32 if out_f32 else torch.bfloat16)
@@ -75,7 +95,7 @@ def _(x, residual, weight, bias, eps, center, out_f32):
     return y, h, x.new_empty(2 if center else 1, x.numel() // D if D else 0, dtype=torch.float32)
 
 
-@torch.library.register_fake("gmdn::norm_bwd")
+@_register_fake("norm_bwd")
 def _(s, stats, weight, dy, dh, center, want_bf16, want_f32, want_w, want_b):
     def out(wanted, dtype, shape):
         return s.new_empty(shape if wanted else (0,), dtype=dtype)
@@ -151,7 +171,7 @@ class TokenLogprobs(NamedTuple):
     top_ids: Optional[Tensor]        # (..., top_k) int64
 
 
-@torch.library.register_fake("gmdn::token_logprobs_fwd")
+@_register_fake("token_logprobs_fwd")
 def _(logits, targets, entropy, top_k, ignore_index):
     shape = logits.shape[:-1]
 
@@ -163,7 +183,7 @@ def _(logits, targets, entropy, top_k, ignore_index):
             logits.new_empty(*shape, 4, dtype=torch.float32))
 
 
-@torch.library.register_fake("gmdn::token_logprobs_bwd")
+@_register_fake("token_logprobs_bwd")
 def _(logits, targets, ids, stats, g_lp, g_ent, g_top, ignore_index):
     return logits.new_empty(logits.shape)
 
@@ -232,24 +252,24 @@ def _codes_like(x):
             x.new_empty((x.numel() + BLOCK8 - 1) // BLOCK8, dtype=torch.float32))
 
 
-@torch.library.register_fake("gmdn::pack8")
+@_register_fake("pack8")
 def _(x):
     return _codes_like(x)
 
 
-@torch.library.register_fake("gmdn::unpack8")
+@_register_fake("unpack8")
 def _(codes, scales, f32):
     return codes.new_empty(codes.shape, dtype=torch.float32 if f32 else torch.bfloat16)
 
 
-@torch.library.register_fake("gmdn::act8_fwd")
+@_register_fake("act8_fwd")
 def _(x, gate):
     codes, scales = _codes_like(x)
     g = (codes.new_empty(0), scales.new_empty(0)) if gate is None else _codes_like(x)
     return x.new_empty(x.shape), codes, scales, *g
 
 
-@torch.library.register_fake("gmdn::act8_bwd")
+@_register_fake("act8_bwd")
 def _(codes, scales, gcodes, gscales, dy, restore):
     return (dy.new_empty(dy.shape), dy.new_empty(dy.shape if gcodes is not None else 0),
             dy.new_empty(dy.shape if restore else 0))
