@@ -99,6 +99,19 @@ class SwiGLU(nn.Module):
         return self.out(F.silu(self.gate(x)) * self.up(x))
 
 
+def _plain(module: nn.Module, cls: type) -> bool:
+    """Whether calling the module is what cls.forward does, and no more: not a subclass or a
+    wrapper, no hooks, no forward of its own.  Only then may its weights be read in its place."""
+    return (type(module) is cls and "forward" not in module.__dict__
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                     or module._backward_pre_hooks)
+            and not nn.modules.module._has_any_global_hook())
+
+
+def _plain_linear(module: nn.Module) -> bool:
+    return _plain(module, nn.Linear) and module.bias is None
+
+
 class Block(nn.Module):
     def __init__(self, d_model: int, n_heads: int, inner: str, chunk: int, ns_steps: int,
                  mixer_cls=MixerLayer, mlp: str = "gelu", act8: bool = False):
@@ -119,12 +132,21 @@ class Block(nn.Module):
         x = x + self.mixer(self.n1(x))
         return x + self.mlp_forward(self.n2(x))
 
+    def mlp_weights(self):
+        """(up, down, gate or None) of an MLP that ``mlp8`` computes, else None."""
+        m = self.mlp
+        if _plain(m, SwiGLU):
+            if all(_plain_linear(p) for p in (m.gate, m.up, m.out)):
+                return m.up.weight, m.out.weight, m.gate.weight
+        elif _plain(m, nn.Sequential) and len(m) == 3:
+            if _plain(m[1], nn.GELU) and m[1].approximate == "none" and _plain_linear(m[0]) \
+                    and _plain_linear(m[2]):
+                return m[0].weight, m[2].weight, None
+        return None
+
     def mlp_forward(self, x):
-        if not self.act8:
-            return self.mlp(x)
-        gate = self.mlp.gate.weight if isinstance(self.mlp, SwiGLU) else None
-        up = self.mlp[0].weight if gate is None else self.mlp.up.weight
-        return step_ops.mlp8(x, up, self.mlp[2].weight, gate)
+        weights = self.mlp_weights() if self.act8 else None
+        return self.mlp(x) if weights is None else step_ops.mlp8(x, *weights)
 
     def forward_fused(self, x, branch):
         """The block on a stream x whose last branch is not yet added (None:
@@ -136,7 +158,11 @@ class Block(nn.Module):
 
 def fused_norm(norm: nn.RMSNorm, x: torch.Tensor, branch):
     """(norm(x + branch), x + branch) in one pass; the normalised output in the
-    autocast type, which is what the projections after it read."""
+    autocast type, which is what the projections after it read.  A norm that is
+    not a plain nn.RMSNorm is called."""
+    if not _plain(norm, nn.RMSNorm):
+        x = x if branch is None else x + branch
+        return norm(x), x
     dt = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
     if branch is None:
         return step_ops.rms_norm(x, norm.weight, None, norm.eps, out_dtype=dt), x
@@ -152,6 +178,9 @@ class LanguageModel(nn.Module):
     autocast type).  act8: the MLPs keep their activations in 8 bits for the
     backward, 5.2 instead of 18 bytes a token and model channel under bf16
     autocast, at a relative error of about 1 % in their weight gradients.
+    Both read the weights of the blocks, norms and MLPs made here in place of
+    calling them; a module that was replaced, wrapped or given hooks is called,
+    and that part of the model runs as without the option.
     """
 
     def __init__(self, vocab: int, d_model: int, n_layers: int, n_heads: int, inner: str,
@@ -181,7 +210,10 @@ class LanguageModel(nn.Module):
         if self.fused:
             branch = None
             for blk in self.blocks:
-                x, branch = blk.forward_fused(x, branch)
+                if _plain(blk, Block):
+                    x, branch = blk.forward_fused(x, branch)
+                else:
+                    x, branch = blk(x if branch is None else x + branch), None
             return self.lm_head(fused_norm(self.norm_f, x, branch)[0])
         for blk in self.blocks:
             x = blk(x)
