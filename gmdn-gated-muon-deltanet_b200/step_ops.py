@@ -25,6 +25,7 @@ arguments' checks and the public names.
 
 from __future__ import annotations
 
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -345,13 +346,18 @@ def _has_tangent(*tensors: Optional[Tensor]) -> bool:
     return any(t is not None and unpack_dual(t).tangent is not None for t in tensors)
 
 
+def _rows(t: Tensor) -> Tensor:
+    """(..., D) as a matrix; a D of 0 leaves nothing to infer the rows from."""
+    return t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+
+
 class _Mlp8Function(torch.autograd.Function):
     """down(act(up x)) that keeps x and the activation's inputs in 8 bits; the
     weight gradients are products with the restored tensors."""
 
     @staticmethod
     def forward(ctx, x, w_up, w_down, w_gate):
-        rows = x.reshape(-1, x.shape[-1])
+        rows = _rows(x)
         up = F.linear(rows, w_up)
         y, saved = act8_forward(up, None if w_gate is None else F.linear(rows, w_gate))
         kept = pack8(rows) if w_up.requires_grad or (w_gate is not None and w_gate.requires_grad) \
@@ -378,7 +384,7 @@ class _Mlp8Function(torch.autograd.Function):
         gate = Packed8(*more[:2], ctx.dtype) if ctx.gated else None
         saved = Act8Saved(Packed8(codes, scales, ctx.dtype), gate)
         need = ctx.needs_input_grad
-        dout = dout.reshape(-1, dout.shape[-1]).to(ctx.dtype)
+        dout = _rows(dout).to(ctx.dtype)
         dup, dgate, y = act8_backward(saved, dout @ w_down, restore=need[2])
         dx = dw_up = dw_gate = dw_down = None
         if need[2]:

@@ -98,3 +98,20 @@ def test_norm_with_only_h_used(x_dt, res_dt, D):
         (dx,) = torch.autograd.grad(
             call(leaves[0], residual=leaves[1].detach())[1], leaves[0], dh)
         assert torch.equal(dx, dh.to(x_dt))
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_mlp8_of_no_width(gated):
+    """A width of 0 anywhere: the shapes and zeros that nn.Linear gives."""
+    pkg = load_pkg()
+    for lead in ((5,), (2, 3), ()):
+        for D, Fh, Do in ((0, 8, 4), (4, 0, 3), (4, 8, 0), (0, 0, 0)):
+            ps = [torch.randn(s, generator=_gen(5)).cuda().requires_grad_(True)
+                  for s in ((*lead, D), (Fh, D), (Do, Fh), (Fh, D))[:4 if gated else 3]]
+            out = pkg.mlp8(*ps)
+            assert out.shape == (*lead, Do) and not out.any()
+            grads = torch.autograd.grad(out, ps, torch.ones_like(out))
+            for g, p in zip(grads, ps):
+                assert g.shape == p.shape and not g.any()
+            with torch.no_grad():
+                assert pkg.mlp8(*ps).shape == out.shape
