@@ -115,3 +115,77 @@ def test_mlp8_of_no_width(gated):
                 assert g.shape == p.shape and not g.any()
             with torch.no_grad():
                 assert pkg.mlp8(*ps).shape == out.shape
+
+
+def _half_step(v, dtype):
+    """Half the distance between the type's numbers around v (of the subnormal ones below)."""
+    e = torch.floor(torch.log2(v.abs().clamp_min(2.0 ** -126)))
+    return torch.exp2(e) * U(dtype)
+
+
+def _tails(dtype):
+    """Arguments of both signs where P, the sigmoid and their products stay normal numbers."""
+    x = torch.cat([torch.linspace(-13, 13, 1 << 14), torch.linspace(-3, 3, 1 << 12)])
+    # blocks of 128 around one magnitude, so that the 8-bit values are as far out as the input's
+    return x.sort().values.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_gelu_keeps_its_digits_on_the_small_side(dtype):
+    """Relative to y, dx and the restored y themselves.  P is within 5.4e-5 (bf16: the fit) or
+    8e-7 (fp32: see the fp32 test of y) of its value, e^(-x^2 / 2) within 2^-22 and, for bf16,
+    two roundings of its exponent, x^2 / 2 EPS each; then at most 8 fp32 roundings of terms no
+    larger than P and |x| phi, and the output's own.  Below 2^-126 the exponential is 0."""
+    pkg = load_pkg()
+    x = _tails(dtype)
+    rel = 5.4e-5 if dtype == BF else 8e-7   # beyond the roundings counted in check()
+
+    def share(v):
+        return torch.special.erfc(-v / math.sqrt(2.0)) / 2
+
+    def check(got, want, terms, exponent, what):
+        fp32 = 8 * EPS * terms + 2.0 ** -126 * 16
+        _within(got, want, exponent + fp32 + _half_step(want, dtype) * (1 + 2.0 ** -8), what)
+
+    def parts(v):
+        v = v.double()
+        phi = torch.exp(-v * v / 2) / math.sqrt(2 * math.pi)
+        e_err = 2.0 ** -22 + (v * v * EPS if dtype == BF else 0.0)
+        return v, share(v), phi, (rel + e_err) * share(v), e_err * phi
+
+    y, saved = pkg.act8_forward(x.cuda())
+    v, P, phi, P_err, phi_err = parts(x)
+    check(y, v * P, v.abs() * P, v.abs() * P_err, "y")
+    dx, _, back = pkg.act8_backward(saved, torch.ones_like(x).cuda())
+    v, P, phi, P_err, phi_err = parts(so.unpack8(*so.pack8(x)).float())
+    check(back, v * P, v.abs() * P, v.abs() * P_err, "restored y")
+    check(dx, P + v * phi, P + v.abs() * phi, P_err + v.abs() * phi_err, "dx")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_swiglu_keeps_its_digits_on_the_small_side(dtype):
+    """Relative: the sigmoid is 1 / (1 + e^-a), off by 2^-21 and, for bf16, by the rounding of
+    its exponent, |a| 2 EPS (log2 e and the product); dgate's slope is the sum of sig, silu and
+    -silu sig.  A sigmoid below 2^-126 is 0."""
+    pkg = load_pkg()
+    a = torch.cat([_tails(dtype).float() * 6, _tails(dtype).float()]).sort().values.to(dtype)
+    u = torch.linspace(0.5, 3.0, a.numel()).to(dtype)
+    y, saved = pkg.act8_forward(u.cuda(), a.cuda())
+    dx, dgate, back = pkg.act8_backward(saved, torch.ones_like(u).cuda())
+
+    def parts(t):
+        t = t.double()
+        sig = torch.sigmoid(t)
+        return t, sig, 2.0 ** -21 + (2 * EPS * t.abs() if dtype == BF else 0.0)
+
+    def check(got, want, size, rel, what):
+        _within(got, want, size * (rel + 8 * EPS) + 2.0 ** -125 * 300
+                + _half_step(want, dtype) * (1 + 2.0 ** -8), what)
+
+    t, sig, rel = parts(a)
+    check(y, t * sig * u.double(), (t * sig * u.double()).abs(), rel, "y")
+    t, sig, rel = parts(so.unpack8(*so.pack8(a)).float())
+    w = so.unpack8(*so.pack8(u)).float().double()
+    check(back, t * sig * w, (t * sig * w).abs(), rel, "restored y")
+    check(dx, t * sig, (t * sig).abs(), rel, "dx")
+    check(dgate, w * sig * (1 + t * (1 - sig)), w * sig * (1 + 2 * t.abs()), 2 * rel, "dgate")
