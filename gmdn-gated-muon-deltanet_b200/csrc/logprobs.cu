@@ -61,6 +61,7 @@ static_assert(kList >= kMaxCluster * kMaxTopK, "rank 0 joins the cluster's lists
 // before, and 0 * -inf, or a sum of S times a mask's -3e38, is not a number.
 constexpr float kFar = -1000.f;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2eLow = 1.925962991e-08f;   // what fp32 leaves of log2 e
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -518,7 +519,8 @@ __global__ void __launch_bounds__(kMaxThreads) logprobs_fwd_kernel(LogprobArgs p
   if (writer) {
     const float H = bad ? nan : (empty ? 0.f : ls - a.q / a.s);
     if (p.stats)
-      reinterpret_cast<float4*>(p.stats)[r] = make_float4(a.m, bad ? nan : ls, kEnt ? H : nan, 0.f);
+      reinterpret_cast<float4*>(p.stats)[r] = make_float4(a.m, bad ? nan : ls, kEnt ? H : nan,
+                                                            bad ? nan : a.s);
     if (p.entropy) p.entropy[r] = H;
     if (p.logprobs)
       p.logprobs[r] = t == p.ignore_index ? 0.f : (t >= 0 && t < p.vocab ? logprob(xt) : nan);
@@ -658,12 +660,28 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(LogprobArgs p
   const bool zero = ls == -INFINITY ||
                     (gl == 0.f && gh == 0.f && !(kTop && __any_sync(~0u, any_top)));
   const float A = kEnt ? -fmaf(gh, st.z, wsum) : -wsum, B = -gh;
+  // 1 / S where a gradient's fp32 digits need it (stats made by hand may leave S at 0)
+  const float inv = sizeof(T) == 4 ? (st.w > 0.f ? __fdiv_rn(1.f, st.w) : expf(-ls)) : 0.f;
   auto grad2 = [&](float2 v) {
-    float2 lp = __fadd2_rn(__fadd2_rn(v, pair(-m)), pair(-ls));
-    const float2 y = __fmul2_rn(lp, pair(kLog2e));
-    const float2 e = make_float2(ex2(y.x), ex2(y.y));
+    float2 c = __fadd2_rn(v, pair(-m)), e, lp;
+    if constexpr (sizeof(T) == 4) {
+      // p = e^c / S: e^(c - log S) would round its exponent twice, |logprob| 2^-24 each, and the
+      // product with log2 e once more; here its rounding, and that of log2 e, goes into the
+      // exponential as 1 + l log 2.  A NaN row has NaN in S.
+      c = make_float2(fmaxf(c.x, kFar), fmaxf(c.y, kFar));
+      const float2 y = __fmul2_rn(c, pair(kLog2e));
+      float2 l = __ffma2_rn(c, pair(kLog2e), make_float2(-y.x, -y.y));
+      l = __ffma2_rn(c, pair(kLog2eLow), l);
+      e = make_float2(ex2(y.x), ex2(y.y));
+      e = __fmul2_rn(e, __ffma2_rn(l, pair(inv * 0.6931471805599453f), pair(inv)));
+      lp = __fadd2_rn(c, pair(-ls));   // at least kFar - log S
+    } else {
+      lp = __fadd2_rn(c, pair(-ls));
+      const float2 y = __fmul2_rn(lp, pair(kLog2e));
+      e = make_float2(ex2(y.x), ex2(y.y));
+    }
     if constexpr (kEnt) {
-      lp = make_float2(fmaxf(lp.x, kFar), fmaxf(lp.y, kFar));
+      if constexpr (sizeof(T) == 2) lp = make_float2(fmaxf(lp.x, kFar), fmaxf(lp.y, kFar));
       return __fmul2_rn(e, __ffma2_rn(lp, pair(B), pair(A)));
     }
     return __fmul2_rn(e, pair(A));

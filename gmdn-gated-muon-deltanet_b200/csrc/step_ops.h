@@ -41,7 +41,7 @@ struct LogprobArgs {
   bool f32;
   const int64_t* targets;        // (batch, length), may be null (forward)
   int64_t ignore_index;
-  float* stats;                  // (rows, 4): max, log of the sum, entropy, target's logprob
+  float* stats;                  // (rows, 4): max, log of the sum, entropy, the sum
   float *logprobs, *entropy, *top_logprobs;   // any may be null
   int64_t* top_ids;              // (rows, top_k)
   int top_k;

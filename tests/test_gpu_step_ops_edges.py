@@ -189,3 +189,32 @@ def test_swiglu_keeps_its_digits_on_the_small_side(dtype):
     check(back, t * sig * w, (t * sig * w).abs(), rel, "restored y")
     check(dx, t * sig, (t * sig).abs(), rel, "dx")
     check(dgate, w * sig * (1 + t * (1 - sig)), w * sig * (1 + 2 * t.abs()), 2 * rel, "dgate")
+
+
+@pytest.mark.parametrize("V", [400, 401])
+def test_logprobs_fp32_gradient_keeps_its_digits(V):
+    """The gradient's -p relative to itself, down to e^-85, in EPS: the exponential 4 (2^-22) and
+    its correction 2; 1 / S and the products 3; S: a thread's chunk, a warp's and the warps'
+    joins 14 adds, and the exponentials of the columns that make it, 4 + 1.5 |c| each.  The logits
+    are multiples of 2^-8, so x - max is exact.  Below 2^-126 the exponential is 0."""
+    pkg = load_pkg()
+    z = torch.round(torch.rand(64, V, generator=_gen(V)) * -90 * 256) / 256
+    z[:, 7] = 2.0
+    t = torch.full((64,), 7)
+    zg = z.cuda().requires_grad_(True)
+    got = pkg.token_logprobs(zg, t.cuda(), entropy=True)
+    lp = torch.log_softmax(z.double(), -1)
+    p = lp.exp()
+    c = z.double() - z.double().amax(-1, keepdim=True)
+    s_err = 14 + 4 + 1.5 * (p * c.abs()).sum(-1, keepdim=True)
+    rel = (s_err + 4 + 2 + 3) * EPS
+    tiny = 2.0 ** -126
+    others = torch.arange(V) != 7
+    (g,) = torch.autograd.grad(got.logprobs.sum(), zg, retain_graph=True)
+    _within(g.cpu()[:, others], -p[:, others], (p * rel + tiny)[:, others], "-p")
+    # the entropy's: p (logprob + H) with log S, the logprob and H off by 2 EPS of themselves each
+    H = -(p * lp).sum(-1, keepdim=True)
+    (g,) = torch.autograd.grad(got.entropy.sum(), zg)
+    size = lp.abs() + H + torch.log(torch.exp(c).sum(-1, keepdim=True)).abs()
+    _within(g, -p * (lp + H), p * size * (rel + 8 * EPS) + p * (s_err * EPS * 4) + 100 * tiny,
+            "entropy")
