@@ -33,7 +33,9 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
+// The runtime's last error is taken too: what is reported here is not the next call's.
 int cuda_fail(cudaError_t e, const char* where) {
+  (void)cudaGetLastError();
   return fail(GMDN_ERR_CUDA, "%s: %s", where, cudaGetErrorString(e));
 }
 

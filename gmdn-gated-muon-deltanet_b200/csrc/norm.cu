@@ -544,18 +544,22 @@ int slots_of(Shape sh) { return sh.lanes > 0 ? kRowThreads / sh.lanes : 1; }
 // One wave of CTAs (kPair: of clusters, two CTAs each), each walking rows a grid apart;
 // for odd widths the step is a multiple of 8 rows.
 template <typename K>
-int wave(K kernel, long long rows, Shape sh, size_t smem) {
+cudaError_t wave(K kernel, long long rows, Shape sh, size_t smem, int* out) {
   const int slots = slots_of(sh);
   const long long want = (rows + slots - 1) / slots;
   long long grid = want;
   if (sh.lanes == kPair) {
     int n = 0;
     ClusterLaunch at(2 * kSms, sh.threads, smem, nullptr);
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &at.cfg) != cudaSuccess || n < 8) n = 8;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &at.cfg);
+    if (e != cudaSuccess) return e;
+    if (n < 8) n = 8;   // an odd width's step is a multiple of 8 rows
     if (n < grid) grid = n;
   } else if (want > kSms) {
     int n = 1;
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, sh.threads, smem);
+    const cudaError_t e =
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, sh.threads, smem);
+    if (e != cudaSuccess) return e;
     const long long cap = static_cast<long long>(kSms) * (n < 1 ? 1 : n);
     if (cap < grid) grid = cap;
   }
@@ -563,7 +567,8 @@ int wave(K kernel, long long rows, Shape sh, size_t smem) {
     const int per = 8 / slots > 0 ? 8 / slots : 1;
     grid = grid / per * per;
   }
-  return static_cast<int>(grid);
+  *out = static_cast<int>(grid);
+  return cudaSuccess;
 }
 
 // 48 KB, the kernel's own `buf` counted, is what a launch may use without being asked for more.
@@ -728,9 +733,11 @@ cudaError_t fwd_go(const NormFwdArgs& p, Shape sh, cudaStream_t st) {
   auto k = norm_fwd_regs<TX, TR, NV, LPR, kOdd, R>;
   const size_t copy = Place<NV, LPR, kOdd>::copy_floats(p.width) * sizeof(float) * slots_of(sh);
   const size_t smem = kOdd ? copy * ((p.weight ? 1 : 0) + (p.bias ? 1 : 0)) : 0;
+  int grid = 0;
   cudaError_t e = allow(k, smem);
+  if (e == cudaSuccess) e = wave(k, p.rows, sh, smem, &grid);
   if (e != cudaSuccess) return e;
-  k<<<wave(k, p.rows, sh, smem), sh.threads, smem, st>>>(p);
+  k<<<grid, sh.threads, smem, st>>>(p);
   return cudaGetLastError();
 }
 template <typename TX, typename TR, bool kOdd>
@@ -758,9 +765,10 @@ cudaError_t bwd_go(const NormBwdArgs& p, Shape sh, int most, int* parts, cudaStr
   const size_t copies = kOdd && p.weight ? Place<NV, LPR, kOdd>::copy_floats(p.width) * slots : 0;
   const size_t sums = LPR > 0 && (p.dw || p.db) ? static_cast<size_t>(p.width) * slots : 0;
   const size_t smem = sizeof(float) * (copies > sums ? copies : sums);
+  int grid = 0;
   cudaError_t e = allow(k, smem);
+  if (e == cudaSuccess) e = wave(k, p.rows, sh, smem, &grid);
   if (e != cudaSuccess) return e;
-  int grid = wave(k, p.rows, sh, smem);
   if (grid > most) grid = most;   // a multiple of 8
   *parts = grid;
   if constexpr (LPR == kPair) {

@@ -56,3 +56,21 @@ def test_norm_abi_refuses_a_dh_of_another_type(width, s_f32):
     assert "type of s" in lib.gmdn_last_error_string().decode()
     assert bwd(FAKE, s_f32) == 1 and bwd(NULL, 1 - s_f32) == 1   # refused for their size alone
     assert "negative size" in lib.gmdn_last_error_string().decode()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers are not a device's")
+@pytest.mark.parametrize("width", [64, 768, 2048, 1283, 16384, 12345, 40000])
+def test_without_a_device_every_launch_is_an_error(width):
+    """Occupancy queries and launches fail and say so; a call after them starts clean."""
+    lib = load_pkg()._lib.lib
+    for _ in range(2):
+        assert lib.gmdn_norm_fwd(FAKE, NULL, FAKE, FAKE, FAKE, NULL, FAKE, FAKE, 10000, width, 1e-5, 1,
+                                 0, 0, 0, NULL) == 4
+        assert "norm_fwd" in lib.gmdn_last_error_string().decode()
+        for dw in (FAKE, NULL):
+            need = lib.gmdn_norm_bwd_workspace_bytes(10000, width)
+            assert lib.gmdn_norm_bwd(FAKE, FAKE, FAKE, FAKE, FAKE, NULL, FAKE, NULL, dw, NULL, FAKE,
+                                     need, 10000, width, 1, 0, 0, 0, 0, 0, NULL) == 4
+            assert "norm_bwd" in lib.gmdn_last_error_string().decode()
+        assert lib.gmdn_norm_fwd(NULL, NULL, NULL, NULL, NULL, NULL, NULL, NULL, 0, width, 1e-5, 1, 0,
+                                 0, 0, NULL) == 0
