@@ -445,6 +445,8 @@ int gmdn_norm_bwd(const void* s, const float* rstd, const float* mean, const flo
   const size_t need = gmdn_norm_bwd_workspace_bytes(rows, width);
   if ((dweight || dbias) && (!workspace || workspace_bytes < need))
     return fail(GMDN_ERR_WORKSPACE, "workspace %zu bytes < required %zu", workspace_bytes, need);
+  if ((dweight || dbias) && misaligned({workspace}))
+    return fail(GMDN_ERR_INVALID, "norm: workspace must be 16-byte aligned");
   gmdn::NormBwdArgs p{s, rstd, mean, weight, dy, dh, ds_a, ds_b, dweight, dbias,
                       static_cast<float*>(workspace), rows, width, center != 0, s_f32 != 0,
                       dy_f32 != 0, a_f32 != 0, b_f32 != 0};

@@ -241,7 +241,7 @@ int gmdn_norm_fwd(const void* x, const void* residual, const float* weight, cons
                   void* y, void* h, float* rstd, float* mean, long long rows, int width, float eps,
                   int center, int x_f32, int res_f32, int y_f32, void* stream);
 
-/* Scratch bytes for gmdn_norm_bwd when it computes dweight or dbias. */
+/* Scratch bytes (16-byte aligned) for gmdn_norm_bwd when it computes dweight or dbias. */
 size_t gmdn_norm_bwd_workspace_bytes(long long rows, int width);
 
 /* Backward: s is what was normalised (x, or h), dy the cotangent of y, dh that

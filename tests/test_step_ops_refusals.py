@@ -74,3 +74,12 @@ def test_without_a_device_every_launch_is_an_error(width):
             assert "norm_bwd" in lib.gmdn_last_error_string().decode()
         assert lib.gmdn_norm_fwd(NULL, NULL, NULL, NULL, NULL, NULL, NULL, NULL, 0, width, 1e-5, 1, 0,
                                  0, 0, NULL) == 0
+
+
+def test_norm_abi_refuses_a_misaligned_workspace():
+    lib = load_pkg()._lib.lib
+    need = lib.gmdn_norm_bwd_workspace_bytes(1000, 768)
+    for at in (0x1001, 0x1002, 0x1004, 0x1008):
+        assert lib.gmdn_norm_bwd(FAKE, FAKE, FAKE, FAKE, FAKE, NULL, FAKE, NULL, FAKE, NULL,
+                                 ctypes.c_void_p(at), need, 1000, 768, 1, 0, 0, 0, 0, 0, NULL) == 1
+        assert "workspace" in lib.gmdn_last_error_string().decode()
