@@ -8,7 +8,8 @@ import torch.autograd.forward_ad as fw
 
 from conftest import load_pkg
 from oracle import step_oracle as so
-from test_gpu_step_ops import BF, EPS, FP, U, _check_norm, _gen, _norm_case, _within
+from test_gpu_step_ops import (BF, EPS, FP, U, _check_logprobs, _check_norm, _gen, _norm_case,
+                               _within)
 
 pytestmark = pytest.mark.gpu
 
@@ -218,3 +219,110 @@ def test_logprobs_fp32_gradient_keeps_its_digits(V):
     size = lp.abs() + H + torch.log(torch.exp(c).sum(-1, keepdim=True)).abs()
     _within(g, -p * (lp + H), p * size * (rel + 8 * EPS) + p * (s_err * EPS * 4) + 100 * tiny,
             "entropy")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("V", [64, 1001, 5003, 32000])
+def test_logprobs_of_the_views_themselves(dtype, V):
+    """Rows at every alignment, read in place: outputs and the gradient (whose rows lie at
+    another alignment) element by element against the oracle, with entropy and alternatives."""
+    pkg = load_pkg()
+    base = (torch.randn(15, V + 9, generator=_gen(V)) * 3).to(dtype)
+    cb = base.cuda()
+    t = torch.randint(0, V, (15,), generator=_gen(1))
+    t[4] = -100
+    for off in range(9 if dtype == BF else 5):
+        view = cb[:, off:off + V]
+        seen = []
+
+        class Calls:      # the call that the check makes, with the tensor that it is given
+            @staticmethod
+            def token_logprobs(z, *args, **kw):
+                seen.append((z.data_ptr(), z.stride()))
+                return pkg.token_logprobs(z, *args, **kw)
+
+        for k in (0, 6):
+            _check_logprobs(Calls, base[:, off:off + V], t, k, cuda_z=view)
+        assert seen == [(view.data_ptr(), (V + 9, 1))] * 2
+        # the same rows as a shifted batch: equal bits
+        cube = cb.view(3, 5, V + 9)[:, :-1, off:off + V]
+        keep = [r for r in range(15) if r % 5 != 4]
+        flat = view.detach().requires_grad_(True)
+        zg = cube.detach().requires_grad_(True)
+        assert zg.data_ptr() == view.data_ptr() and zg.stride() == (5 * (V + 9), V + 9, 1)
+        for kw in (dict(entropy=True, top_k=6), dict(entropy=True), dict(top_k=3), dict()):
+            a = pkg.token_logprobs(flat, t.cuda(), **kw)
+            b = pkg.token_logprobs(zg, t[keep].view(3, 4).cuda(), **kw)
+            cots = [torch.randn(x.shape, generator=_gen(7)).cuda() for x in a[:3] if x is not None]
+            for x, y in zip(a, b):
+                assert (x is None) == (y is None)
+                assert x is None or torch.equal(x[keep], y.reshape(12, *y.shape[2:]))
+            (ga,) = torch.autograd.grad([x for x in a[:3] if x is not None], flat, cots)
+            (gb,) = torch.autograd.grad([x for x in b[:3] if x is not None], zg,
+                                        [c[keep].view(3, 4, *c.shape[1:]) for c in cots])
+            assert torch.equal(ga[keep], gb.reshape(12, V))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("rows, V, parts", [(160, 20003, 1), (2, 131073, 8)])
+def test_logprobs_alternatives_in_few_threads(dtype, rows, V, parts):
+    """Large logits that fall to 40 of the 128 groups of threads which give the bound: it is
+    then taken from the others, and more columns lie above it than are listed (1024)."""
+    pkg = load_pkg()
+    E = 16 // dtype.itemsize     # elements of a 16-byte chunk
+    z = torch.randn(rows, V, generator=_gen(V))
+    col = torch.arange(V)
+    most = []
+    for r in range(rows):
+        off = r * V % E                              # where the row starts in its first chunk
+        chunk = (col + off) // E
+        per = -(-((off + V - 1) // E + 1) // parts)
+        raised = chunk % per % 128 < 40
+        z[r, raised] = 20.0 + torch.rand(int(raised.sum()), generator=_gen(r)) * 10
+        most.append(int((raised & (chunk < per)).sum()))
+    assert min(most) > 1024
+    z = z.to(dtype)              # bf16: about a hundred values, hundreds of ties each
+    t = torch.randint(0, V, (rows,), generator=_gen(3))
+    _check_logprobs(pkg, z, t, 64, grads=rows < 10)
+    _check_logprobs(pkg, z, t, 7, grads=False)
+
+
+def test_odd_and_wide_rows_in_a_captured_graph():
+    """Shared memory beyond 48 KB, clusters of two CTAs and of eight, captured and replayed on
+    new inputs: equal to plain calls."""
+    pkg = load_pkg()
+    cases = []
+    for D in (1283, 6101, 8192, 12101, 16384):
+        c = _norm_case(200, D, True, FP, BF, BF)
+        cases.append({n: c[n].cuda().requires_grad_(n in ("x", "res", "w", "b"))
+                      for n in ("x", "res", "w", "b", "dy", "dh")})
+    z = torch.randn(4, 50021, generator=_gen(1)).cuda().requires_grad_(True)
+    t = torch.randint(0, 50021, (4,), generator=_gen(2)).cuda()
+
+    def step():
+        out = []
+        for c in cases:
+            y, h = pkg.layer_norm(c["x"], c["w"], c["b"], residual=c["res"], out_dtype=BF)
+            out += [y.detach(), *torch.autograd.grad([y, h], [c[n] for n in ("x", "res", "w", "b")],
+                                                     [c["dy"], c["dh"]])]
+        got = pkg.token_logprobs(z, t, entropy=True, top_k=20)
+        loss = got.logprobs.sum() + got.entropy.sum() + got.top_logprobs.sum()
+        return out + [got.top_ids, loss.detach(), *torch.autograd.grad(loss, [z])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        z.neg_()
+        for c in cases:
+            c["x"].mul_(-1.5)
+    graph.replay()
+    want = step()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
