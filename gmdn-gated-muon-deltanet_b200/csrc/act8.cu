@@ -17,8 +17,8 @@
 // Memory bounds it, with the instruction slots close: bf16 GELU moves 5 bytes an
 // element forward and 7 backward, which leaves ~27 and ~38 instructions an
 // element at the copy rate; the kernels take 19.  Measured (B200): 16384 x 4096
-// bf16 GELU 60 us forward (0.86 of the 6536 GB/s copy rate) and 86 backward
-// (0.84), SwiGLU at 0.88 and more, fp32 GELU at 0.88 and 0.83.
+// bf16 GELU 59 us forward (0.86 of the 6536 GB/s copy rate) and 85 backward
+// (0.84), SwiGLU at 0.85 and more, fp32 GELU at 0.87 and 0.84.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -68,7 +68,8 @@ __device__ __forceinline__ float2 neg2(float2 a) { return make_float2(-a.x, -a.y
 // nothing cancels; beyond, the form above with more terms, in t = 1 / (1 + 0.3 |x|),
 // and with e's exponent in two parts, since its rounding is a relative error of x^2 / 2
 // half ulps.  R and the terms are weighted least-squares fits (reweighted towards
-// the smallest largest error) to the functions in fp64: 7e-10 and 2e-8 relative.
+// the smallest largest error) to the functions in fp64: with the coefficients as fp32
+// numbers 3.4e-8 and 2.4e-8 relative.
 // P is within 8e-7 of its value relative (largest seen: 3.8e-7), rounding and the
 // SFU's 2^-22 included, on the small side too (subnormal P is 0).  About 18
 // instructions an element:

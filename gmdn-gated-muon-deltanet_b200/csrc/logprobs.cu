@@ -33,8 +33,8 @@
 // would use 0.7 of the SFUs' rate for bf16.  Products and sums go two to an
 // instruction, rescaling by a new maximum is a branch that few chunks take, and
 // a warp's threads meet over one common maximum.  Measured (B200): 16376 x 32000
-// bf16 with entropy 183 us (0.88 of the 6536 GB/s copy rate), its gradient 363
-// us (0.88); 4 x 32000 fp32 with 20 alternatives 8 us, 24 x 256000 with 64 17 us;
+// bf16 with entropy 183 us (0.88 of the 6536 GB/s copy rate), its gradient 358
+// us (0.90); 4 x 32000 fp32 with 20 alternatives 8 us, 24 x 256000 with 64 17 us;
 // 4096 x 32000 with 20 alternatives 81 us against 53 without any.
 
 #include <cooperative_groups.h>

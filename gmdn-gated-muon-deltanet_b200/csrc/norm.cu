@@ -17,9 +17,13 @@
 // 8 to 16 bytes.  So a row is read once and held in registers from its first
 // sum to its last output, and dw, db are summed in registers over all of a
 // thread's rows.  Measured (B200, copy rate 6536 GB/s): 16384 x 768, fp32 stream
-// and bf16 branch: forward 26 us (0.90 of the copy rate), backward 42 us (0.73,
-// with the 5 us join of the CTAs' column sums); 8192 x 4096 and wider fp32 rows
-// 0.87 to 0.92 both ways; 8192 x 8192 bf16 96 and 112 us (0.86, 0.73).
+// and bf16 branch: forward 26 us (0.89 of the copy rate), backward 42 us (0.73,
+// with the 5 us join of the CTAs' column sums); 8192 x 8192 bf16 layer norm 96
+// and 114 us (0.86, 0.72); RMS norm of fp32 rows of 4096 and 8192 elements 0.85 to
+// 0.91 both ways.  A layer norm of such rows waits for two sums a row: fp32 8192 x
+// 8192 119 and 148 us (0.69, 0.83), 4897 x 13704 154 and 231 (0.53, 0.53).  The
+// backward is lowest at 1024, where it writes the most partials: 16384 rows of
+// fp32 42 us (0.61).
 
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -204,11 +208,10 @@ struct Place {
       }
     }
   }
-  // whether the row reaches into group v, lies all over it, and its elements there
+  // whether the row reaches into group v, and its elements there
   __device__ __forceinline__ bool has(int v) const {
     return kOdd ? mask[kOdd ? v : 0] != 0 : group(v) * 8 < width;
   }
-  __device__ __forceinline__ bool whole(int v) const { return !kOdd || mask[kOdd ? v : 0] == 0xffu; }
   __device__ __forceinline__ uint32_t bits(int v) const { return kOdd ? mask[kOdd ? v : 0] : 0xffu; }
   __device__ __forceinline__ int group(int v) const { return v * tpr + tid; }
   // the row's first group as an element of the tensor
