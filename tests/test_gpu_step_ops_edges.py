@@ -326,3 +326,85 @@ def test_odd_and_wide_rows_in_a_captured_graph():
     want = step()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_logprobs_gradient_from_stats_without_the_sum():
+    """Stats whose fourth number is 0: 1 / S is e^(-log S), off by the logarithm's rounding."""
+    load_pkg()
+    ops = torch.ops.gmdn
+    z = torch.randn(5, 300, generator=_gen(1)).cuda()
+    t = torch.tensor([0, 299, -100, 7, 8]).cuda()
+    stats = ops.token_logprobs_fwd(z, t, True, 0, -100)[4]
+    g = torch.randn(5, generator=_gen(2)).cuda()
+    want = ops.token_logprobs_bwd(z, t, None, stats, g, g, None, -100)
+    stats[:, 3] = 0.0
+    got = ops.token_logprobs_bwd(z, t, None, stats, g, g, None, -100)
+    # log S ~ 4 rounded to 2^-22 / 2, expf 2 ulp; a gradient's terms are below |g| (1 + |lp| + H)
+    assert (got - want).abs().max() <= 16 * EPS * g.abs().max()
+
+
+def _small_block(pkg):
+    g = _gen(9)
+    w, w1, w2 = (torch.randn(s, generator=g).cuda().requires_grad_(True)
+                 for s in ((64,), (96, 64), (64, 96)))
+
+    def loss(x, t):
+        y, h = pkg.rms_norm(x, w, residual=x)
+        y = pkg.mlp8(y, w1, w2) + h
+        got = pkg.token_logprobs(y, t, entropy=True, top_k=2)
+        return got.entropy.mean() - got.logprobs.mean()
+    x = torch.randn(7, 64, generator=g).cuda().requires_grad_(True)
+    t = torch.randint(0, 64, (7,), generator=g).cuda()
+    return loss, x, t, [x, w, w1, w2]
+
+
+def test_saved_tensors_elsewhere_and_recomputed():
+    """Saved tensors moved to the host and back, and a forward run again in the backward."""
+    from torch.utils.checkpoint import checkpoint
+    loss, x, t, leaves = _small_block(load_pkg())
+    want = torch.autograd.grad(loss(x, t), leaves)
+    with torch.autograd.graph.save_on_cpu():
+        a = loss(x, t)
+    for got in (torch.autograd.grad(a, leaves),
+                torch.autograd.grad(checkpoint(loss, x, t, use_reentrant=False), leaves)):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_compiled_for_any_number_of_rows():
+    torch._dynamo.reset()
+    loss, _, _, (_, *weights) = _small_block(load_pkg())
+    compiled = torch.compile(loss, dynamic=True)
+    for n in (3, 5, 130, 1):
+        x = torch.randn(n, 64, generator=_gen(n)).cuda()
+        t = torch.randint(0, 64, (n,), generator=_gen(n)).cuda()
+        for a, b in zip(torch.autograd.grad(compiled(x, t), weights),
+                        torch.autograd.grad(loss(x, t), weights)):
+            # the plain parts may add in another order, and move a code by one
+            assert (a - b).norm() <= 2e-2 * b.norm() + 1e-12
+
+
+def test_threads_on_their_own_streams():
+    import threading
+    loss, x, t, leaves = _small_block(load_pkg())
+    want = torch.autograd.grad(loss(x, t), leaves)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(10):
+                    got = torch.autograd.grad(loss(x, t), leaves)
+                    s.synchronize()
+                    if not all(torch.equal(p, q) for p, q in zip(got, want)):
+                        wrong.append(i)
+        except Exception as e:   # noqa: BLE001 - reported below
+            wrong.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
